@@ -283,6 +283,95 @@ int mpsa_gemm_block_scaled_batched(const void* a, const void* a_scale, const voi
                                    int batch, int M, int N, int K, int mode, int a_fmt, int b_fmt, int out_dtype,
                                    float alpha, int* status, void* stream);
 
+/* ---- serving token by token ----
+ * None of the entries below has a counterpart in the reference, which sees whole sequences in 16 bits on every call
+ * (ours/mxfp_attn_kernel.py:19-74). */
+
+/* RMS norm of queries and keys and their rotation by position, one launch for both.  For every row x of D elements (one head of one token)
+ *   y = x / sqrt(mean(x^2) + eps) * weight        norm 1: the mean over the row, weight [D]; norm 2: over all the token's heads, weight [H*D]
+ *   pair i of the first `rot` elements turned by the angle whose cosine and sine are cos / sin[position, i]
+ * in fp32, rounded once.  Pair i is (y[i], y[i + rot/2]), or with interleaved (y[2i], y[2i + 1]); elements from `rot` on are not rotated.
+ *   x, y       [B,H,L,D], element strides, innermost dense; strides multiples of 4, bases of 4 elements.  x[1] null: one operand.
+ *              y may be x itself with the same strides.
+ *   weight     null: no weight.  w_dtype as in_dtype, each operand's own
+ *   cos, sin   fp32 [table_rows, rot/2], 16-byte aligned; null: no rotation (rot is then ignored)
+ *   positions  int32 (pos64 0) or int64 (1) [B or 1, L, axes], batch stride pos_sb; null: token l has position l (one axis).  With
+ *              several axes pair i goes by the axis a with section_end[a-1] <= i < section_end[a].
+ *              A token with a position outside the table gets NaN in its rotated elements. */
+typedef struct mpsa_norm_rope_args {
+  const void* x[2];
+  void* y[2];
+  const void* weight[2];
+  long long x_sb[2], x_sh[2], x_sl[2], y_sb[2], y_sh[2], y_sl[2];
+  const void *cos, *sin, *positions;
+  long long pos_sb, table_rows;
+  int H[2], w_dtype[2], section_end[4];
+  int in_dtype, B, L, D, rot, norm, axes, interleaved, pos64;
+  float eps;
+} mpsa_norm_rope_args;
+int mpsa_norm_rope(const mpsa_norm_rope_args* args, void* stream);
+
+/* A paged cache of keys and values in MX blocks of 32 along the depth.
+ *   k, v              element codes [num_pages, Hkv, page_size, D] bytes (elem 0 E4M3, 1 E5M2), or D/2 bytes with two E2M1 codes each, the
+ *                     lower depth in the low half (elem 2)
+ *   k_scale, v_scale  scale codes [num_pages, Hkv, page_size, D/32]: element = code * 2^(scale - 127), 255 is NaN
+ *   page_size         a power of two from 16 to 1024; D 64 or 128; all four dense and 16-byte aligned
+ * A sequence's token t is in row t % page_size of page page_table[b, t / page_size] (int32 [B, max_pages], batch stride table_sb).  Entries
+ * outside [0, num_pages) stand for no page: nothing is written there, and keys there are not seen. */
+typedef struct mpsa_kv_cache {
+  void *k, *v, *k_scale, *v_scale;
+  int num_pages, page_size, Hkv, D, elem;
+} mpsa_kv_cache;
+
+/* Quantises new tokens into the cache.  Token t of sequence b goes to position start[b] + t if t < counts[b] (counts null: all T) and
+ * the page table reaches that far.  A block's scale is the smallest power of two (2^-126 at least) at which no element exceeds the type's
+ * largest value; elements are rounded to nearest even.  A block with a NaN or an infinity gets scale 255 and zero codes.
+ *   k, v   [B,Hkv,T,D] of in_dtype, element strides that are multiples of 8, 16-byte aligned bases
+ * Two tokens of one call that fall on one row of one page (a page listed twice) leave either or a mixture. */
+typedef struct mpsa_kv_append_args {
+  mpsa_kv_cache cache;
+  const void *k, *v;
+  long long k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, table_sb;
+  const int *page_table, *start, *counts;
+  int in_dtype, B, T, max_pages;
+} mpsa_kv_append_args;
+int mpsa_kv_append(const mpsa_kv_append_args* args, void* stream);
+
+/* Reads sequences back: k_out, v_out dense [B,Hkv,max_len,D] of out_dtype, 16-byte aligned; rows from lengths[b] on, and rows without a
+ * page, are zero. */
+typedef struct mpsa_kv_read_args {
+  mpsa_kv_cache cache;
+  void *k_out, *v_out;
+  long long table_sb;
+  const int *page_table, *lengths;
+  int out_dtype, B, max_len, max_pages;
+} mpsa_kv_read_args;
+int mpsa_kv_read(const mpsa_kv_read_args* args, void* stream);
+
+/* Attention of the last tokens of each sequence over the cache that holds them: softmax(q k^T sm_scale) v in fp32 over the cached values,
+ * P rounded to fp16.  Sequence b has lengths[b] keys, of which the last q_lens[b] (null: T) belong to its queries.  A query sees every key before those; of
+ * those, query i sees key j iff j <= i, or with a mask iff mask[b,i,j] != 0.
+ *   q, out    [B,Hq,T,D], 16-bit, element strides, innermost dense (q: strides multiples of 8, 16-byte aligned; out the same)
+ *   mask      bytes [B or 1, T, T], batch stride mask_sb, dense rows
+ *   lse       optional fp32 [B,Hq,T] dense: log2 of each row's softmax denominator, as in mpsa_attn_fwd
+ *   workspace mpsa_kv_attention_workspace bytes, 256-byte aligned, private to the call until it has finished on the GPU
+ * Rows that see no key, and rows from q_lens[b] on, give zero (lse -inf). */
+typedef struct mpsa_kv_attention_args {
+  mpsa_kv_cache cache;
+  const void* q;
+  void* out;
+  void* lse;
+  void* workspace;
+  long long workspace_bytes;
+  long long q_sb, q_sh, q_sl, o_sb, o_sh, o_sl, table_sb, mask_sb;
+  const int *page_table, *lengths, *q_lens;
+  const unsigned char* mask;
+  int dtype, B, T, Hq, max_pages;
+  float sm_scale;
+} mpsa_kv_attention_args;
+long long mpsa_kv_attention_workspace(const mpsa_kv_attention_args* args);
+int mpsa_kv_attention(const mpsa_kv_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

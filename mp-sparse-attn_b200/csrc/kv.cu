@@ -1,0 +1,200 @@
+// The paged MX cache of keys and values: quantised as it is written (mpsa_kv_append) and read back (mpsa_kv_read).  See include/mpsa.h for
+// the layout.  Both are memory traffic: every element is read once and written once.
+#include "api_internal.h"
+#include "common.cuh"
+#include "serving.cuh"
+
+namespace mpsa {
+
+int check_cache(const mpsa_kv_cache& c, const char* what) {
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale) return set_error(MPSA_ERR_BAD_ARG, "%s: null cache pointer", what);
+  if (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.k_scale | (uintptr_t)c.v_scale) % 16)
+    return set_error(MPSA_ERR_BAD_ARG, "%s: the cache must be 16-byte aligned", what);
+  if (c.elem < 0 || c.elem > 2) return set_error(MPSA_ERR_BAD_ARG, "%s: elem must be 0 (E4M3), 1 (E5M2) or 2 (E2M1)", what);
+  if (c.D != 64 && c.D != 128) return set_error(MPSA_ERR_UNSUPPORTED, "%s: D must be 64 or 128", what);
+  if (c.num_pages <= 0 || c.Hkv <= 0 || c.Hkv > 65535) return set_error(MPSA_ERR_BAD_ARG, "%s: the cache needs pages and 1 to 65535 heads", what);
+  if (c.page_size < 16 || c.page_size > 1024 || (c.page_size & (c.page_size - 1)))
+    return set_error(MPSA_ERR_UNSUPPORTED, "%s: page_size must be a power of two from 16 to 1024", what);
+  return MPSA_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 128;
+
+template <int ELEM> struct Largest;
+template <> struct Largest<E4M3> { static constexpr int exponent = 8; static constexpr uint32_t mantissa = 0x600000; };     // 448
+template <> struct Largest<E5M2> { static constexpr int exponent = 15; static constexpr uint32_t mantissa = 0x600000; };    // 57344
+template <> struct Largest<E2M1> { static constexpr int exponent = 2; static constexpr uint32_t mantissa = 0x400000; };     // 6
+
+// The smallest power of two at which amax (bits) does not exceed the type's largest value, as its exponent.
+template <int ELEM>
+__device__ __forceinline__ int block_exponent(uint32_t amax) {
+  const int e = (int)(amax >> 23) - 127 - Largest<ELEM>::exponent + ((amax & 0x7fffffu) > Largest<ELEM>::mantissa);
+  return max(e, -126);                     // (and with it every subnormal amax, and zero)
+}
+
+template <int ELEM>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8]) {
+  if constexpr (ELEM == E2M1) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t two;
+      asm("{\n.reg .b8 h;\ncvt.rn.satfinite.e2m1x2.f32 h, %2, %1;\ncvt.u32.u8 %0, h;\n}" : "=r"(two) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+      r |= two << (8 * i);
+    }
+    *reinterpret_cast<uint32_t*>(p) = r;
+  } else {
+    uint32_t r[2] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned short two;
+      if constexpr (ELEM == E4M3) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(two) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+      else asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(two) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+      r[i / 2] |= (uint32_t)two << (16 * (i % 2));
+    }
+    *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  float a[4], b[4];
+  load4(p, a);
+  load4(p + 4, b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+
+// D/8 lanes take a row of K and the same row of V, 8 elements each; 4 lanes share a block of 32.
+template <typename T, int ELEM, int LANES>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ mpsa_kv_append_args a) {
+  constexpr int D = 8 * LANES, NB = D / 32, kRows = kThreads / LANES;
+  const int j = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
+  const int t = blockIdx.x * kRows + threadIdx.x / LANES;
+  const int n = a.counts ? min(a.counts[b], a.T) : a.T;
+  const mpsa_kv_cache& c = a.cache;
+  const long long pos = (long long)a.start[b] + t;
+  const int page = t < n && pos >= 0 && pos < (1ll << 31) ? page_of(a.page_table + b * a.table_sb, (int)(pos / c.page_size), a.max_pages, c.num_pages) : -1;
+  const long long row = ((long long)max(page, 0) * c.Hkv + h) * c.page_size + (pos & (c.page_size - 1));
+  float x[2][8] = {};
+  if (page >= 0) {
+    load8(static_cast<const T*>(a.k) + b * a.k_sb + h * a.k_sh + t * a.k_sl + 8 * j, x[0]);
+    load8(static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh + t * a.v_sl + 8 * j, x[1]);
+  }
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+    uint32_t amax = 0;                                          // as bits: a NaN is the largest
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[o][i]) & 0x7fffffffu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const bool fine = amax < 0x7f800000u;
+    const int e = fine ? block_exponent<ELEM>(amax) : 128;
+    const float r = __uint_as_float((uint32_t)(127 - e) << 23);  // exact: e is -126 .. 126
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[o][i] = fine ? x[o][i] * r : 0.0f;
+    if (page >= 0) {
+      store_codes<ELEM>(static_cast<uint8_t*>(o ? c.v : c.k) + row * code_bytes(ELEM, D) + code_bytes(ELEM, 8 * j), x[o]);
+      if (j % 4 == 0) static_cast<uint8_t*>(o ? c.v_scale : c.k_scale)[row * NB + j / 4] = (uint8_t)(e + 127);
+    }
+  }
+}
+
+template <int ELEM>
+__device__ __forceinline__ void read_codes(const uint8_t* p, float (&x)[8]) {
+  uint32_t w[2];
+  if constexpr (ELEM == E2M1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = ELEM == E2M1 ? w[0] >> (8 * i) : w[i / 2] >> (16 * (i % 2));
+    const float2 f = __half22float2(elem_pair<ELEM>(two));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+template <typename T, int ELEM, int LANES>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ mpsa_kv_read_args a) {
+  constexpr int D = 8 * LANES, NB = D / 32, kRows = kThreads / LANES;
+  const int j = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
+  const int t = blockIdx.x * kRows + threadIdx.x / LANES;
+  if (t >= a.max_len) return;
+  const mpsa_kv_cache& c = a.cache;
+  const int page = t < a.lengths[b] ? page_of(a.page_table + b * a.table_sb, t / c.page_size, a.max_pages, c.num_pages) : -1;
+  const long long row = ((long long)max(page, 0) * c.Hkv + h) * c.page_size + (t & (c.page_size - 1));
+  const long long to = (((long long)b * c.Hkv + h) * a.max_len + t) * D + 8 * j;
+  float x[2][8] = {};
+  if (page >= 0) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      read_codes<ELEM>(static_cast<const uint8_t*>(o ? c.v : c.k) + row * code_bytes(ELEM, D) + code_bytes(ELEM, 8 * j), x[o]);
+      const float s = scale_value(static_cast<const uint8_t*>(o ? c.v_scale : c.k_scale)[row * NB + j / 4]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[o][i] *= s;
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+    T* y = static_cast<T*>(o ? a.v_out : a.k_out) + to;
+    const float lo[4] = {x[o][0], x[o][1], x[o][2], x[o][3]}, hi[4] = {x[o][4], x[o][5], x[o][6], x[o][7]};
+    store4(y, lo);
+    store4(y + 4, hi);
+  }
+}
+
+template <typename T, int ELEM>
+int append_as(const mpsa_kv_append_args& a, cudaStream_t st) {
+  const int rows = kThreads / (a.cache.D / 8);
+  const dim3 grid((a.T + rows - 1) / rows, a.cache.Hkv, a.B);
+  if (a.cache.D == 64) kv_append_kernel<T, ELEM, 8><<<grid, kThreads, 0, st>>>(a);
+  else kv_append_kernel<T, ELEM, 16><<<grid, kThreads, 0, st>>>(a);
+  return check_launch("kv_append");
+}
+template <typename T>
+int append_elem(const mpsa_kv_append_args& a, cudaStream_t st) {
+  return a.cache.elem == E4M3 ? append_as<T, E4M3>(a, st) : a.cache.elem == E5M2 ? append_as<T, E5M2>(a, st) : append_as<T, E2M1>(a, st);
+}
+
+template <typename T, int ELEM>
+int read_as(const mpsa_kv_read_args& a, cudaStream_t st) {
+  const int rows = kThreads / (a.cache.D / 8);
+  const dim3 grid((a.max_len + rows - 1) / rows, a.cache.Hkv, a.B);
+  if (a.cache.D == 64) kv_read_kernel<T, ELEM, 8><<<grid, kThreads, 0, st>>>(a);
+  else kv_read_kernel<T, ELEM, 16><<<grid, kThreads, 0, st>>>(a);
+  return check_launch("kv_read");
+}
+template <typename T>
+int read_elem(const mpsa_kv_read_args& a, cudaStream_t st) {
+  return a.cache.elem == E4M3 ? read_as<T, E4M3>(a, st) : a.cache.elem == E5M2 ? read_as<T, E5M2>(a, st) : read_as<T, E2M1>(a, st);
+}
+
+}  // namespace
+}  // namespace mpsa
+
+using namespace mpsa;
+
+extern "C" int mpsa_kv_append(const mpsa_kv_append_args* a, void* stream) {
+  if (!a || !a->k || !a->v || !a->page_table || !a->start) return set_error(MPSA_ERR_BAD_ARG, "kv_append: null pointer");
+  if (int rc = check_cache(a->cache, "kv_append")) return rc;
+  if (a->in_dtype < 0 || a->in_dtype > 2) return set_error(MPSA_ERR_UNSUPPORTED, "kv_append: inputs must be bf16, fp16 or fp32");
+  if (a->B <= 0 || a->T <= 0 || a->max_pages <= 0) return set_error(MPSA_ERR_BAD_ARG, "kv_append: non-positive shape");
+  if (a->B > 65535) return set_error(MPSA_ERR_UNSUPPORTED, "kv_append: at most 65535 sequences");
+  if ((a->k_sb | a->k_sh | a->k_sl | a->v_sb | a->v_sh | a->v_sl) % 8 || ((uintptr_t)a->k | (uintptr_t)a->v) % 16)
+    return set_error(MPSA_ERR_UNSUPPORTED, "kv_append: k and v need 16-byte aligned bases and strides that are multiples of 8 elements");
+  const cudaStream_t st = (cudaStream_t)stream;
+  return a->in_dtype == 0 ? append_elem<__nv_bfloat16>(*a, st) : a->in_dtype == 1 ? append_elem<__half>(*a, st) : append_elem<float>(*a, st);
+}
+
+extern "C" int mpsa_kv_read(const mpsa_kv_read_args* a, void* stream) {
+  if (!a || !a->k_out || !a->v_out || !a->page_table || !a->lengths) return set_error(MPSA_ERR_BAD_ARG, "kv_read: null pointer");
+  if (int rc = check_cache(a->cache, "kv_read")) return rc;
+  if (a->out_dtype < 0 || a->out_dtype > 2) return set_error(MPSA_ERR_UNSUPPORTED, "kv_read: outputs are fp32, fp16 or bf16");
+  if (a->B <= 0 || a->max_len <= 0 || a->max_pages <= 0) return set_error(MPSA_ERR_BAD_ARG, "kv_read: non-positive shape");
+  if (a->B > 65535) return set_error(MPSA_ERR_UNSUPPORTED, "kv_read: at most 65535 sequences");
+  if (((uintptr_t)a->k_out | (uintptr_t)a->v_out) % 16) return set_error(MPSA_ERR_BAD_ARG, "kv_read: outputs must be 16-byte aligned");
+  const cudaStream_t st = (cudaStream_t)stream;
+  return a->out_dtype == 0 ? read_elem<float>(*a, st) : a->out_dtype == 1 ? read_elem<__half>(*a, st) : read_elem<__nv_bfloat16>(*a, st);
+}

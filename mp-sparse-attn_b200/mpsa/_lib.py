@@ -56,6 +56,11 @@ _SIGNATURES = {
     "mpsa_gemm_block_scaled_batched": ([c_void_p] * 5 + [c_int] * 8 + [c_float, c_void_p, c_void_p], c_int),
     "mpsa_gemm_block_scaled": ([c_void_p] * 5 + [c_int, c_int, c_int, c_ll, c_ll, c_ll, c_int, c_int, c_int, c_int,
                                 c_float, c_void_p, c_void_p], c_int),
+    "mpsa_norm_rope": ([c_void_p, c_void_p], c_int),
+    "mpsa_kv_append": ([c_void_p, c_void_p], c_int),
+    "mpsa_kv_read": ([c_void_p, c_void_p], c_int),
+    "mpsa_kv_attention_workspace": ([c_void_p], c_ll),
+    "mpsa_kv_attention": ([c_void_p, c_void_p], c_int),
 }
 EXPORTS = tuple(_SIGNATURES)
 
