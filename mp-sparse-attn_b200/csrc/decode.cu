@@ -1,21 +1,26 @@
 // Attention of a sequence's last tokens over its paged MX cache (mpsa_kv_attention).
 //
-// A unit of work is one sequence, one KV head and up to 16 of its query rows (row r = token r / G, query head r % G of the KV head's G).
+// A unit of work is one sequence, one KV head and up to 8 NR of its query rows (row r = token r / G, query head r % G of the KV head's G).
 // A step is 32 keys.  The steps of all units, laid end to end, are cut into equal runs, one per CTA, whatever the lengths are: CTAs compute
-// the cut from the lengths in device memory.  A unit that falls to several CTAs leaves parts (fp32 sums with their row maxima and
+// the cut from the lengths in device memory.  A unit that falls to several CTAs leaves parts (fp32 sums with their row references and
 // denominators), which the combining kernel adds up in the order of the keys.
 //
 // Within a CTA the warps take steps in turn and have nothing to do with each other until the run's part of a unit is done: each copies its own
-// keys to its own shared memory with cp.async, and keeps its own maxima, sums and output in registers.
+// keys to its own shared memory with cp.async, and keeps its own references, sums and output in registers.
 //
-//   scores    S = Q K^T by m16n8k16 on fp16 operands.  Element codes convert exactly; a block's 32 depth elements are two instructions of
-//             their own, whose fp32 result is multiplied by the key's scale of that block.  Queries are brought to a largest magnitude of
-//             1 .. 2 by a power of two of their row, so that their 8 or 11 significant bits survive in fp16.
-//   output    O = P V: the block scales of V differ from key to key, so they go to P: for each block of the depth P times the scales is
-//             rounded to fp16 and multiplied by the codes.  The scales enter relative to the largest one so far, 2^15 above it at most: fp16
-//             then keeps 11 bits down to 2^-29 of the largest product.  That rounding of P is the only one below fp32.
+//   scores    S^T = K Q^T by m16n8k16 on fp16 operands, keys in the M dimension: a few query rows fill the N of 8.  Element codes convert
+//             exactly; a block's 32 depth elements are two instructions of their own, whose fp32 result is multiplied by the key's scale of
+//             that block.  Queries are brought to a largest magnitude of 1 .. 2 by a power of two of their row, so that their 8 or 11
+//             significant bits survive in fp16.
+//   output    O^T = V^T P^T, depth in the M dimension.  The block scales of V differ from key to key, so they go to P: for each block of the
+//             depth P times the scales is rounded to fp16 and multiplied by the codes.  This rounding of P is the only one below fp32.
+//   softmax   against a reference U of the row that keeps those products, not P, within fp16: U is set so that the largest (score plus log2
+//             of the key's largest scale) gives 2^7, and raised when one would give more than 2^15.  Products keep 11 bits down to 2^-21 of
+//             the row's largest, whatever the sizes of other keys' values are.  P and the row's sum of P are fp32; U is at least the largest
+//             score - 100, so that they stay finite (values below 2^-90 have fewer bits, then).
+// Fragments of K and V come from ldmatrix on the codes as they are (.trans for V: two keys of neighbouring depth elements in a register).
 //
-// It is bound by the cache's bytes (HBM) as long as the conversions keep up: two ALU-pipe instructions for two elements.
+// It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each.
 #include "api_internal.h"
 #include "common.cuh"
 #include "serving.cuh"
@@ -25,13 +30,16 @@
 namespace mpsa {
 namespace {
 
-constexpr int kWarps = 4, kStep = 32, kRows = 16;
+constexpr int kWarps = 4, kStep = 32;
 constexpr int kMinShare = 4;                   // steps of a run at least: one for each warp
+constexpr float kMost = 15.0f, kSet = 7.0f;    // log2 of the largest product that raises no reference, and of the largest one after a raise
+constexpr int kLeast = -85;                    // log2 of a scale that counts as that at least: references are the largest score - 100 at least
 
 struct Call : mpsa_kv_attention_args {
-  int groups;                                  // row groups of a (sequence, KV head)
-  float* part;                                 // [2 x CTAs][kRows][D], a CTA's run has at most two units that it shares with others
-  float2* stat;                                // [2 x CTAs][kRows]: row maximum (log2), denominator relative to it
+  int tiles;                                   // NR: row tiles of 8 in a unit
+  int groups;                                  // units of a (sequence, KV head)
+  float* part;                                 // [2 x CTAs][8 NR][D], a CTA's run has at most two units that it shares with others
+  float2* stat;                                // [2 x CTAs][8 NR]: row reference (log2), denominator relative to it
 };
 
 __device__ __forceinline__ int length_of(const Call& a, int b) {
@@ -88,70 +96,101 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Shared memory of a warp: kStages steps of [K codes][V codes][K scales][V scales], then the step's scales as floats.
-template <int ELEM, int D>
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {          // an 8 x 8 matrix of 16-bit values, two of a row in a lane
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Shared memory: for each warp kStages steps of [K codes][V codes][K scales][V scales] and the step's scales as floats, then the unit's
+// queries in the order of the fragments and the factors of its rows.  The warps' parts of the output go where the steps were.
+template <int ELEM, int D, int NR>
 struct Layout {
-  static constexpr int row = code_bytes(ELEM, D), nb = D / 32;
+  static constexpr int row = code_bytes(ELEM, D), nb = D / 32, rows = 8 * NR;
   static constexpr int codes = kStep * row, stage = 2 * codes + 2 * kStep * nb;
   static constexpr int stages = 2;
   static constexpr int scales = stages * stage, warp = scales + 2 * kStep * nb * 4;
-  static constexpr int pitch = D + 4;                                  // floats of a row in the merge buffer
-  static constexpr int merge = kWarps * kRows * pitch * 4;
-  static constexpr int bytes = kWarps * warp > merge ? kWarps * warp : merge;
-  // Where a row's block of 32 elements lies: blocks change places so that the lanes of a fragment load meet different banks.  K: 8 rows
-  // at a time, V: rows 2t of the quarter.
-  static constexpr int block = row / nb;                               // bytes
-  static __device__ __forceinline__ int k_swap(int r) { return D == 64 ? (ELEM == E2M1 ? r >> 2 : r >> 1) & 1 : (ELEM == E2M1 ? r >> 1 : r) & 3; }
-  static __device__ __forceinline__ int v_swap(int r) { return D == 64 ? (ELEM == E2M1 ? r >> 2 : r >> 1) & 1 : (r >> 1) & 3; }
+  static constexpr int pitch = D + 8;                                  // floats of a row of a warp's part
+  static constexpr int merge = kWarps * rows * pitch * 4;
+  static constexpr int queries = kWarps * warp > merge ? kWarps * warp : merge;
+  static constexpr int bytes = queries + rows * D * 2 + rows * 4;
+  static constexpr int pairs = row / 32;                               // pieces of 32 bytes of a row: what one ldmatrix takes of 16 keys
+  static_assert(stage % 128 == 0 && warp % 128 == 0 && queries % 128 == 0, "the blocks' places are found by exclusive or");
+  // Where a row's 16-byte pieces lie: the eight rows of a matrix meet different banks.
+  static __device__ __forceinline__ int swap(int r) { return row == 128 ? r & 7 : row == 64 ? (r >> 1) & 3 : (r >> 2) & 1; }
+  // A lane's first depth element in instruction s of a block: four in the order of a fragment of K and Q; two of V^T and O^T
+  static __device__ __forceinline__ int k_depth(int s, int t) { return ELEM == E2M1 ? 8 * t + 4 * s : 16 * s + 4 * t; }
+  static __device__ __forceinline__ int v_depth(int s, int g) { return ELEM == E2M1 ? 4 * g + 2 * s : 16 * s + 2 * g; }
 };
 
-// Eight codes of K (depth 8t .. 8t + 7 of a block), as the fp16 pairs of two instructions' B operands
+// One piece of 32 bytes of 16 keys (K): the A operands of its instructions; 8 bits: one block, 4 bits: two.
 template <int ELEM>
-__device__ __forceinline__ void k_fragments(uint32_t p, uint32_t (&f)[4]) {
-  if constexpr (ELEM == E2M1) {
-    uint32_t w;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(p));
+__device__ __forceinline__ void k_fragments(uint32_t p, uint32_t (&f)[ELEM == E2M1 ? 4 : 2][4]) {
+  uint32_t w[4];
+  ldmatrix(w, p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = bits(elem_pair<ELEM>(w >> (8 * i)));
-  } else {
-    uint32_t w[2];
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(p));
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = bits(elem_pair<ELEM>(w[i / 2] >> (16 * (i % 2))));
-  }
+    for (int x = 0; x < 2; ++x) {
+      const uint32_t v = w[2 * i + x];                 // keys g + 8x
+      if constexpr (ELEM == E2M1) {
+        f[2 * i][x] = bits(elem_pair<ELEM>(v));
+        f[2 * i][2 + x] = bits(elem_pair<ELEM>(v >> 8));
+        f[2 * i + 1][x] = bits(elem_pair<ELEM>(v >> 16));
+        f[2 * i + 1][2 + x] = bits(elem_pair<ELEM>(v >> 24));
+      } else {
+        f[i][x] = bits(elem_pair<ELEM>(v));
+        f[i][2 + x] = bits(elem_pair<ELEM>(v >> 16));
+      }
+    }
 }
 
-// Codes of V for depth 4g .. 4g + 3 of a block at two keys, as four fp16 pairs (one key in each half)
+// The same of V, transposed: rows of A are depth elements, its columns the keys.
 template <int ELEM>
-__device__ __forceinline__ void v_fragments(uint32_t p0, uint32_t p1, int g, uint32_t (&f)[4]) {
-  uint32_t x, y;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(p0));
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(p1));
-  if constexpr (ELEM == E2M1) {                      // the word holds eight depth elements: g odd takes its upper half
-    const uint32_t w = __byte_perm(x, y, g & 1 ? 0x7632 : 0x5410);                 // x's four codes, y's four
-    const uint32_t a = bits(elem_pair<ELEM>(w)), b = bits(elem_pair<ELEM>(w >> 8)), c = bits(elem_pair<ELEM>(w >> 16)), d = bits(elem_pair<ELEM>(w >> 24));
-    f[0] = __byte_perm(a, c, 0x5410); f[1] = __byte_perm(a, c, 0x7632);
-    f[2] = __byte_perm(b, d, 0x5410); f[3] = __byte_perm(b, d, 0x7632);
-  } else {
-    const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);  // x0 y0 x1 y1, x2 y2 x3 y3
-    f[0] = bits(elem_pair<ELEM>(lo)); f[1] = bits(elem_pair<ELEM>(lo >> 16));
-    f[2] = bits(elem_pair<ELEM>(hi)); f[3] = bits(elem_pair<ELEM>(hi >> 16));
-  }
+__device__ __forceinline__ void v_fragments(uint32_t p, uint32_t (&f)[ELEM == E2M1 ? 4 : 2][4]) {
+  uint32_t w[4];
+  ldmatrix_trans(w, p);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint32_t v = w[2 * i + x];                 // keys 8x + 2t (lower half) and 8x + 2t + 1
+      if constexpr (ELEM == E2M1) {
+        const uint32_t a = bits(elem_pair<ELEM>(v)), b = bits(elem_pair<ELEM>(v >> 8)), c = bits(elem_pair<ELEM>(v >> 16)), d = bits(elem_pair<ELEM>(v >> 24));
+        f[2 * i][2 * x] = __byte_perm(a, c, 0x5410);
+        f[2 * i][2 * x + 1] = __byte_perm(a, c, 0x7632);
+        f[2 * i + 1][2 * x] = __byte_perm(b, d, 0x5410);
+        f[2 * i + 1][2 * x + 1] = __byte_perm(b, d, 0x7632);
+      } else {
+        const uint32_t u = __byte_perm(v, 0, 0x3120);
+        f[i][2 * x] = bits(elem_pair<ELEM>(u));
+        f[i][2 * x + 1] = bits(elem_pair<ELEM>(u >> 16));
+      }
+    }
 }
 
-// RH: halves of the 16 rows that are in use (1: at most 8 rows).
-template <typename T, int ELEM, int D, int RH>
-__global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __grid_constant__ Call a) {
-  using Y = Layout<ELEM, D>;
-  constexpr int NB = D / 32, NT = kStep / 8;
+template <typename T, int ELEM, int D, int NR>
+__global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != E2M1 ? 3 : 4) kv_attention_kernel(const __grid_constant__ Call a) {
+  using Y = Layout<ELEM, D, NR>;
+  constexpr int NB = D / 32, NM = kStep / 16;          // blocks of the depth, key tiles of a step
+  constexpr int BP = ELEM == E2M1 ? 2 : 1;             // blocks of a 32-byte piece
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 row_stat[kWarps][kRows];
+  __shared__ float2 row_stat[kWarps][8 * NR];
   const mpsa_kv_cache& c = a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const uint32_t ring = smem_u32(smem) + warp * Y::warp;
   float* const ksc = reinterpret_cast<float*>(smem + warp * Y::warp + Y::scales);
   float* const vsc = ksc + kStep * NB;
+  uint2* const queries = reinterpret_cast<uint2*>(smem + Y::queries);                  // [block][instruction][row tile][lane]
+  float* const factors = reinterpret_cast<float*>(smem + Y::queries + Y::rows * D * 2);
   const int G = a.Hq / c.Hkv, R = a.T * G, units = c.Hkv * a.groups;
+  const uint32_t mat = (lane & 15) * Y::row + ((lane >> 4) ^ Y::swap(lane & 15)) * 16;  // this lane's row address for ldmatrix
 
   grid_dependents_go();
   const long long share = share_of(a, gridDim.x, lane);
@@ -159,58 +198,14 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
   const long long stop = at + share;
   long long begin;
   int b = sequence_at(a, at, begin, lane);
-  bool first_run = true;
-  for (; b < a.B && at < stop;) {
+  for (bool again = false; b < a.B && at < stop; again = true) {
     const int len = length_of(a, b), steps = steps_of(len);
     const long long off = at - begin;
     const int u = (int)(off / steps), s0 = (int)(off % steps), s1 = (int)min((long long)steps, s0 + (stop - at));
-    const int h = u / a.groups, row0 = u % a.groups * kRows;
+    const int h = u / a.groups, row0 = u % a.groups * Y::rows;
     const int ql = queries_of(a, b, len), first = len - ql;
     const int* const table = a.page_table + b * a.table_sb;
-    if (!first_run) __syncthreads();                  // (the merge buffer has been read)
-    first_run = false;
-
-    // queries: this lane's rows g and g + 8, depth 8t .. 8t + 7 of every block
-    uint32_t qf[NB][RH][4];
-    float rs[RH];
-    int token[RH];
-#pragma unroll
-    for (int x = 0; x < RH; ++x) {
-      const int r = row0 + g + 8 * x;
-      token[x] = r < R ? r / G : -1;
-      float q[NB][8];
-      uint32_t amax = 0;
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        if (r < R) {
-          const T* p = static_cast<const T*>(a.q) + (b * a.q_sb + (h * G + r % G) * a.q_sh + token[x] * a.q_sl + 32 * k + 8 * t);
-          float lo[4], hi[4];
-          load4(p, lo);
-          load4(p + 4, hi);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[k][e] = lo[e], q[k][4 + e] = hi[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q[k][e] = 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(q[k][e]) & 0x7fffffffu);
-      }
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int e = min(max((int)(amax >> 23), 1), 253);              // biased exponent of the row
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-      rs[x] = amax >= 0x7f800000u ? __int_as_float(0x7fffffff) : a.sm_scale * 1.44269504f * __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-      for (int k = 0; k < NB; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[k][x][i] = pack2(__half(), q[k][2 * i] * down, q[k][2 * i + 1] * down);
-    }
-
-    float o[NB][4][4] = {}, m[RH], l[RH];
-#pragma unroll
-    for (int x = 0; x < RH; ++x) m[x] = -INFINITY, l[x] = 0.0f;
-    int vref = 0;                                     // largest scale code of V so far
+    if (again) __syncthreads();                       // (the merge buffer has been read)
 
     // pages: a lane holds one of the warp's next 16 steps' two (16 keys each)
     const int mine = (s1 - s0 - warp + kWarps - 1) / kWarps;          // steps of this warp (may be negative)
@@ -235,18 +230,15 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
         for (int i = 0; i < CPR / 2; ++i) {
           const int r = 16 * half + i * RPI + rl;
           const bool there = pg[half] >= 0 && pos + r < len;
-          constexpr int per = Y::block / 16;                          // pieces of a block: 2 (8 bits) or 1
-          const int kd = ((ch / per) ^ Y::k_swap(r)) * Y::block + ch % per * 16, vd = ((ch / per) ^ Y::v_swap(r)) * Y::block + ch % per * 16;
-          copy16(to + r * Y::row + kd, kp + i * 512, there);
-          copy16(to + Y::codes + r * Y::row + vd, vp + i * 512, there);
+          const uint32_t d = to + r * Y::row + (ch ^ Y::swap(i * RPI + rl)) * 16;
+          copy16(d, kp + i * 512, there);
+          copy16(d + Y::codes, vp + i * 512, there);
         }
       }
-      constexpr int SP = 16 * NB / 16;                                // 16-byte pieces of 16 keys' scales
-      if (lane < 4 * SP) {
-        const int half = lane / SP % 2, v = lane / (2 * SP);
-        const int p = half ? p1 : p0;
+      if (lane < 4 * NB) {                                            // 16-byte pieces: NB for 16 keys of K or V
+        const int half = lane / NB % 2, p = half ? p1 : p0;
         const long long row = ((long long)max(p, 0) * c.Hkv + h) * c.page_size + ((pos + 16 * half) & (c.page_size - 1));
-        copy16(to + 2 * Y::codes + lane * 16, static_cast<const uint8_t*>(v ? c.v_scale : c.k_scale) + row * NB + lane % SP * 16, p >= 0);
+        copy16(to + 2 * Y::codes + lane * 16, static_cast<const uint8_t*>(lane >= 2 * NB ? c.v_scale : c.k_scale) + row * NB + lane % NB * 16, p >= 0);
       }
     };
     auto page = [&](int k, int half) { return __shfl_sync(0xffffffffu, pages, 2 * (k % 16) + half); };
@@ -254,6 +246,50 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
     int cur0 = page(0, 0), cur1 = page(0, 1);         // pages of step k
     if (mine > 0) request(0, cur0, cur1);
     asm volatile("cp.async.commit_group;" ::: "memory");
+
+    // queries of the unit in the order of the B fragments: a warp takes row tiles in turn, a lane row g of it
+    for (int n = warp; n < NR; n += kWarps) {
+      const int r = row0 + 8 * n + g;
+      float q[NB][2][4];
+      uint32_t amax = 0;
+      const T* p = static_cast<const T*>(a.q) + (b * a.q_sb + (h * G + r % G) * a.q_sh + (long long)(r / G) * a.q_sl);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (r < R) load4(p + 32 * i + Y::k_depth(s, t), q[i][s]);
+          else q[i][s][0] = q[i][s][1] = q[i][s][2] = q[i][s][3] = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = max(amax, __float_as_uint(q[i][s][e]) & 0x7fffffffu);
+        }
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int e = min(max((int)(amax >> 23), 1), 253);              // biased exponent of the row
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+      if (t == 0) factors[8 * n + g] = amax >= 0x7f800000u ? __int_as_float(0x7fffffff) : a.sm_scale * 1.44269504f * __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          queries[((2 * i + s) * NR + n) * 32 + lane] = make_uint2(pack2(__half(), q[i][s][0] * down, q[i][s][1] * down), pack2(__half(), q[i][s][2] * down, q[i][s][3] * down));
+    }
+    __syncthreads();
+    float rs[NR][2], m[NR][2], l[NR][2];              // rows 8n + 2t and + 1
+    uint2 qf[NR <= 2 ? 2 * NB : 1][NR <= 2 ? NR : 1];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        rs[n][x] = factors[8 * n + 2 * t + x];
+        m[n][x] = -INFINITY;
+        l[n][x] = 0.0f;
+      }
+      if constexpr (NR <= 2)
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) qf[i][n] = queries[(i * NR + n) * 32 + lane];
+    }
+    float o[NB][2][NR][4] = {};                       // depth v_depth(s, g) (elements 0, 1: rows 2t, 2t + 1) and the next one (2, 3)
+
     for (int k = 0; k < mine; ++k) {
       int nx0 = -1, nx1 = -1;
       if (k + 1 < mine) {
@@ -268,9 +304,11 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
       __syncwarp();
       const int pos = kStep * (s0 + warp + k * kWarps);
       const uint32_t buf = ring + k % Y::stages * Y::stage;
-      const bool special = pos + kStep > (R > 1 && a.T > 1 || a.mask ? first : len) || cur0 < 0 || cur1 < 0;
+      const bool special = pos + kStep > (a.T > 1 || a.mask ? first : len) || cur0 < 0 || cur1 < 0;     // some key not seen by some row
 
       // scales of key `lane`, as floats for everybody
+      bool strange;                                   // a scale of V is NaN
+      float size;                                     // log2 of key `lane`'s largest scale of V
       {
         const bool there = pos + lane < len && (lane < 16 ? cur0 : cur1) >= 0;
         uint32_t kb, vb;
@@ -285,146 +323,175 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
           vb = y;
         }
         if (!there) kb = vb = 0;
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const uint32_t e = vb >> (8 * i) & 255u;
-          top = max(top, e == 255u ? 0u : e);
-        }
-        const int up = max((int)__reduce_max_sync(0xffffffffu, top), vref);
-        if (up > vref) {                              // (for the whole warp)
-          const int d = up - vref;
-          const float f = d > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - d) << 23);
-#pragma unroll
-          for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
-          vref = up;
-        }
+        uint32_t e[NB], top = 0;
         float kf[NB], vf[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
+          e[i] = vb >> (8 * i) & 255u;
+          top = max(top, e[i]);
           kf[i] = scale_value(kb >> (8 * i) & 255u);
-          const uint32_t e = vb >> (8 * i) & 255u;
-          vf[i] = e == 255u ? __int_as_float(0x7fffffff) : e == 0u ? 0.0f : __uint_as_float((uint32_t)max((int)e - vref + 142, 0) << 23);
+          vf[i] = __uint_as_float(e[i] << 23);
         }
+        strange = __any_sync(0xffffffffu, top == 255u);
+        if (strange) {
+          top = 0;
 #pragma unroll
-        for (int i = 0; i < NB; i += 2) {
-          *reinterpret_cast<float2*>(ksc + lane * NB + i) = make_float2(kf[i], kf[i + 1]);
-          *reinterpret_cast<float2*>(vsc + lane * NB + i) = make_float2(vf[i], vf[i + 1]);
+          for (int i = 0; i < NB; ++i) {
+            if (e[i] == 255u) vf[i] = __int_as_float(0x7fffffff);
+            else top = max(top, e[i]);
+          }
+        }
+        size = (float)max((int)top - 127, kLeast);
+        if constexpr (NB == 4) {
+          reinterpret_cast<float4*>(ksc)[lane] = make_float4(kf[0], kf[1], kf[2], kf[3]);
+          reinterpret_cast<float4*>(vsc)[lane] = make_float4(vf[0], vf[1], vf[2], vf[3]);
+        } else {
+          reinterpret_cast<float2*>(ksc)[lane] = make_float2(kf[0], kf[1]);
+          reinterpret_cast<float2*>(vsc)[lane] = make_float2(vf[0], vf[1]);
         }
         __syncwarp();
       }
 
-      // scores in log2 units: s[n][..] is row g, keys 8n + 2t and + 1, then row g + 8
-      float s[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float k0[NB], k1[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          k0[i] = ksc[(8 * n + 2 * t) * NB + i];
-          k1[i] = ksc[(8 * n + 2 * t + 1) * NB + i];
+      // s[w][n][..]: key 16w + g of rows 2t, 2t + 1 of tile n, then key 16w + g + 8
+      float s[NM][NR][4] = {};
+      auto scale_of = [&](const float* p, int key, float (&f)[NB]) {
+        if constexpr (NB == 4) {
+          const float4 v = reinterpret_cast<const float4*>(p)[key];
+          f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        } else {
+          const float2 v = reinterpret_cast<const float2*>(p)[key];
+          f[0] = v.x; f[1] = v.y;
         }
-        const int r = 8 * n + g;
-        const uint32_t kp = buf + r * Y::row;
+      };
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+      for (int w = 0; w < NM; ++w) {
+        float k0[NB], k1[NB];
+        scale_of(ksc, 16 * w + g, k0);
+        scale_of(ksc, 16 * w + g + 8, k1);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          uint32_t f[4];
-          k_fragments<ELEM>(kp + (i ^ Y::k_swap(r)) * Y::block + t * (Y::block / 4), f);
-          float d[4] = {};
-          mma(d, qf[i][0][0], RH > 1 ? qf[i][RH - 1][0] : 0u, qf[i][0][1], RH > 1 ? qf[i][RH - 1][1] : 0u, f[0], f[1]);
-          mma(d, qf[i][0][2], RH > 1 ? qf[i][RH - 1][2] : 0u, qf[i][0][3], RH > 1 ? qf[i][RH - 1][3] : 0u, f[2], f[3]);
+        for (int j = 0; j < Y::pairs; ++j) {
+          uint32_t f[2 * BP][4];
+          k_fragments<ELEM>((buf + 16 * w * Y::row + mat) ^ (32 * j), f);
 #pragma unroll
-          for (int x = 0; x < RH; ++x) {
-            s[n][2 * x] = fmaf(d[2 * x], k0[i], s[n][2 * x]);
-            s[n][2 * x + 1] = fmaf(d[2 * x + 1], k1[i], s[n][2 * x + 1]);
+          for (int i = 0; i < BP; ++i) {
+            const int blk = BP * j + i;
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              float d[4] = {};
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint2 q = NR <= 2 ? qf[NR <= 2 ? 2 * blk + x : 0][NR <= 2 ? n : 0] : queries[((2 * blk + x) * NR + n) * 32 + lane];
+                mma(d, f[2 * i + x][0], f[2 * i + x][1], f[2 * i + x][2], f[2 * i + x][3], q.x, q.y);
+              }
+              s[w][n][0] = fmaf(d[0], k0[blk], s[w][n][0]);
+              s[w][n][1] = fmaf(d[1], k0[blk], s[w][n][1]);
+              s[w][n][2] = fmaf(d[2], k1[blk], s[w][n][2]);
+              s[w][n][3] = fmaf(d[3], k1[blk], s[w][n][3]);
+            }
           }
         }
-#pragma unroll
-        for (int x = 0; x < RH; ++x) {
-          s[n][2 * x] *= rs[x];
-          s[n][2 * x + 1] *= rs[x];
-        }
       }
+
+      // scores in log2 units, and whether a reference has to be raised
+      bool above = false;
+      float sz[NM][2];
+#pragma unroll
+      for (int w = 0; w < NM; ++w) {
+        sz[w][0] = __shfl_sync(0xffffffffu, size, 16 * w + g);
+        sz[w][1] = __shfl_sync(0xffffffffu, size, 16 * w + g + 8);
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int w = 0; w < NM; ++w)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[w][n][x] *= rs[n][x & 1];
       if (special) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int p = pos + 8 * n + 2 * t + e, j = p - first;
-            const bool there = p < len && (n < 2 ? cur0 : cur1) >= 0;
+          for (int x = 0; x < 2; ++x) {
+            const int r = row0 + 8 * n + 2 * t + x, tok = r / G;
+            const bool real = r < R && tok < ql;
+            const unsigned char* const mk = a.mask + b * a.mask_sb + (long long)tok * a.T;
 #pragma unroll
-            for (int x = 0; x < RH; ++x) {
-              const bool seen = there && (j < 0 || (token[x] >= 0 && token[x] < ql && (a.mask ? a.mask[b * a.mask_sb + (long long)token[x] * a.T + j] != 0 : j <= token[x])));
-              if (!seen) s[n][2 * x + e] = -INFINITY;
-            }
-          }
-      }
-
-      // running maxima, probabilities, sums
+            for (int w = 0; w < NM; ++w)
 #pragma unroll
-      for (int x = 0; x < RH; ++x) {
-        float up = m[x];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) up = fmaxf(up, fmaxf(s[n][2 * x], s[n][2 * x + 1]));
-        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
-        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
-        const float ref = up == -INFINITY ? 0.0f : up;
-        if (__any_sync(0xffffffffu, up > m[x])) {
-          const float f = exp2_fast(m[x] - ref);
-          l[x] *= f;
-#pragma unroll
-          for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o[i][j][2 * x] *= f;
-              o[i][j][2 * x + 1] *= f;
-            }
-          m[x] = up;
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          s[n][2 * x] = exp2_fast(s[n][2 * x] - ref);
-          s[n][2 * x + 1] = exp2_fast(s[n][2 * x + 1] - ref);
-          l[x] += s[n][2 * x] + s[n][2 * x + 1];
-        }
-      }
-
-      // O += P V, 16 keys at a time: keys 16w + 2t, + 1, + 8, + 9
-#pragma unroll
-      for (int w = 0; w < kStep / 16; ++w) {
-        const int k0 = 16 * w + 2 * t;
-        const uint32_t vp = buf + Y::codes;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const float v[4] = {vsc[k0 * NB + i], vsc[(k0 + 1) * NB + i], vsc[(k0 + 8) * NB + i], vsc[(k0 + 9) * NB + i]};
-          float p[2][RH][2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int x = 0; x < RH; ++x)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float q = s[2 * w + y][2 * x + e];
-                p[y][x][e] = q * v[2 * y + e];
-                if (special && q == 0.0f) p[y][x][e] = 0.0f;          // (a scale that is NaN, of a key that the row does not see)
+              for (int y = 0; y < 2; ++y) {
+                const int p = pos + 16 * w + g + 8 * y, j = p - first;
+                const bool seen = p < len && (w ? cur1 : cur0) >= 0 && (j < 0 || (real && (a.mask ? mk[j] != 0 : j <= tok)));
+                if (!seen) s[w][n][2 * y + x] = -INFINITY;
               }
-          const uint32_t a0 = pack2(__half(), p[0][0][0], p[0][0][1]), a2 = pack2(__half(), p[1][0][0], p[1][0][1]);
-          const uint32_t a1 = RH > 1 ? pack2(__half(), p[0][RH - 1][0], p[0][RH - 1][1]) : 0u, a3 = RH > 1 ? pack2(__half(), p[1][RH - 1][0], p[1][RH - 1][1]) : 0u;
-          uint32_t f[2][4];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = k0 + 8 * y;                                 // (rows r and r + 1 have their blocks in the same places)
-            const uint32_t pl = vp + r * Y::row + (i ^ Y::v_swap(r)) * Y::block + (ELEM == E2M1 ? 4 * (g / 2) : 4 * g);
-            v_fragments<ELEM>(pl, pl + Y::row, g, f[y]);
           }
+      }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma(o[i][j], a0, a1, a2, a3, f[0][j], f[1][j]);
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float top = fmaxf(fmaxf(s[0][n][x] + sz[0][0], s[0][n][2 + x] + sz[0][1]), fmaxf(s[1][n][x] + sz[1][0], s[1][n][2 + x] + sz[1][1]));
+          above |= top > m[n][x] + kMost;
+        }
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float top = fmaxf(fmaxf(s[0][n][x] + sz[0][0], s[0][n][2 + x] + sz[0][1]), fmaxf(s[1][n][x] + sz[1][0], s[1][n][2 + x] + sz[1][1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kSet;
+            if (top > m[n][x]) {
+              const float f = exp2_fast(m[n][x] - top);
+              l[n][x] *= f;
+#pragma unroll
+              for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  o[i][y][n][x] *= f;
+                  o[i][y][n][2 + x] *= f;
+                }
+              m[n][x] = top;
+            }
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float ref = m[n][x] == -INFINITY ? 0.0f : m[n][x];
+#pragma unroll
+          for (int w = 0; w < NM; ++w) {
+            s[w][n][x] = exp2_fast(s[w][n][x] - ref);
+            s[w][n][2 + x] = exp2_fast(s[w][n][2 + x] - ref);
+            l[n][x] += s[w][n][x] + s[w][n][2 + x];
+          }
+        }
+
+      // O^T += V^T P^T, 16 keys at a time
+#pragma unroll
+      for (int w = 0; w < NM; ++w) {
+        float v0[NB], v1[NB];
+        scale_of(vsc, 16 * w + g, v0);
+        scale_of(vsc, 16 * w + g + 8, v1);
+#pragma unroll
+        for (int j = 0; j < Y::pairs; ++j) {
+          uint32_t f[2 * BP][4];
+          v_fragments<ELEM>((buf + Y::codes + 16 * w * Y::row + mat) ^ (32 * j), f);
+#pragma unroll
+          for (int i = 0; i < BP; ++i) {
+            const int blk = BP * j + i;
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              float p[4] = {s[w][n][0] * v0[blk], s[w][n][1] * v0[blk], s[w][n][2] * v1[blk], s[w][n][3] * v1[blk]};
+              if (special && strange)                 // NaN of a key that the row does not see
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  if (s[w][n][x] == 0.0f) p[x] = 0.0f;
+              const uint32_t b0 = transposed(pack2(__half(), p[0], p[1])), b1 = transposed(pack2(__half(), p[2], p[3]));
+#pragma unroll
+              for (int x = 0; x < 2; ++x) mma(o[blk][x][n], f[2 * i + x][0], f[2 * i + x][1], f[2 * i + x][2], f[2 * i + x][3], b0, b1);
+            }
+          }
         }
       }
       __syncwarp();                                   // the step's buffers are free
@@ -434,26 +501,28 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
-    // the warps' parts together: o[i][j] holds depth 32i + 8t + j and + 4 of rows g and g + 8
+    // the warps' parts together
     float* const merge = reinterpret_cast<float*>(smem);
-    const float back = scale_value(vref) * 0x1p-15f;
 #pragma unroll
-    for (int x = 0; x < RH; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (t == 0) row_stat[warp][g + 8 * x] = make_float2(m[x], l[x]);
-      float* const to = merge + (warp * kRows + g + 8 * x) * Y::pitch + 8 * t;
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int x = 0; x < 2; ++x) {
+        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
+        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
+        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+        const int r = 8 * n + 2 * t + x;
+        if (g == 0) row_stat[warp][r] = make_float2(m[n][x], l[n][x]);
+        float* const to = merge + (warp * Y::rows + r) * Y::pitch;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(to + 32 * i + 4 * e) =
-              make_float4(o[i][0][2 * x + e] * back, o[i][1][2 * x + e] * back, o[i][2][2 * x + e] * back, o[i][3][2 * x + e] * back);
-    }
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            *reinterpret_cast<float2*>(to + 32 * i + Y::v_depth(s, g)) = make_float2(o[i][s][n][x], o[i][s][n][2 + x]);
+      }
     __syncthreads();
     const bool whole = s0 == 0 && s1 == steps;
     const long long slot = 2ll * blockIdx.x + (s0 == 0);
-    for (int i = threadIdx.x; i < 8 * RH * (D / 4); i += 32 * kWarps) {
+    for (int i = threadIdx.x; i < Y::rows * (D / 4); i += 32 * kWarps) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       if (row0 + r >= R) continue;
       float top = -INFINITY;
@@ -465,7 +534,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = exp2_fast(row_stat[w][r].x - ref);
-        const float4 y = *reinterpret_cast<const float4*>(merge + (w * kRows + r) * Y::pitch + d);
+        const float4 y = *reinterpret_cast<const float4*>(merge + (w * Y::rows + r) * Y::pitch + d);
         sum += f * row_stat[w][r].y;
         v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
       }
@@ -477,8 +546,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3) kv_attention_kernel(const __gr
         store4(static_cast<T*>(a.out) + (b * a.o_sb + hq * a.o_sh + tok * a.o_sl + d), y);
         if (a.lse && d == 0) static_cast<float*>(a.lse)[((long long)b * a.Hq + hq) * a.T + tok] = none ? -INFINITY : top + log2f(sum);
       } else {
-        *reinterpret_cast<float4*>(a.part + (slot * kRows + r) * D + d) = v;
-        if (d == 0) a.stat[slot * kRows + r] = make_float2(top, sum);
+        *reinterpret_cast<float4*>(a.part + (slot * Y::rows + r) * D + d) = v;
+        if (d == 0) a.stat[slot * Y::rows + r] = make_float2(top, sum);
       }
     }
     at += s1 - s0;
@@ -494,7 +563,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_constant__ Call a, int ctas) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, units = a.cache.Hkv * a.groups;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
-  const int r = blockIdx.y * kWarps + warp, G = a.Hq / a.cache.Hkv, row = u % a.groups * kRows + r;
+  const int rows = 8 * a.tiles, r = blockIdx.y * kWarps + warp, G = a.Hq / a.cache.Hkv, row = u % a.groups * rows + r;
   const long long share = share_of(a, ctas, lane);
   long long begin = 0;
   for (int i = lane; i < b; i += 32) begin += (long long)steps_of(length_of(a, i)) * units;
@@ -506,13 +575,13 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
   grid_dependency_wait();                             // (by everybody: what follows on the stream counts on it)
   if (c0 == c1 || row >= a.T * G) return;
   float top = -INFINITY, sum = 0.0f;
-  for (long long i = c0; i <= c1; ++i) top = fmaxf(top, a.stat[(2 * i + (i == c0)) * kRows + r].x);
+  for (long long i = c0; i <= c1; ++i) top = fmaxf(top, a.stat[(2 * i + (i == c0)) * rows + r].x);
   const float ref = top == -INFINITY ? 0.0f : top;
   constexpr int N = D / 32;
   float v[N] = {};
 #pragma unroll 4
   for (long long i = c0; i <= c1; ++i) {
-    const long long at = (2 * i + (i == c0)) * kRows + r;
+    const long long at = (2 * i + (i == c0)) * rows + r;
     const float2 st = a.stat[at];
     const float f = exp2_fast(st.x - ref);
     sum += f * st.y;
@@ -539,34 +608,31 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
   if (a.lse && lane == 0) static_cast<float*>(a.lse)[((long long)b * a.Hq + hq) * a.T + tok] = none ? -INFINITY : top + log2f(sum);
 }
 
-constexpr int kPerSm = 3;
-
-int ctas_of(const Call& a) {
+int ctas_of(const Call& a) {                          // of an SM: as many as registers and shared memory let in
   const long long most = (long long)a.B * a.cache.Hkv * a.groups * (((long long)a.max_pages * a.cache.page_size + kStep - 1) / kStep + 1);
-  const long long all = (long long)kPerSm * sm_count();
+  const long long all = (a.tiles == 4 ? 2ll : a.tiles == 2 || a.cache.elem != E2M1 ? 3ll : 4ll) * sm_count();
   return (int)(most < all ? most : all);
 }
 
-template <typename T, int ELEM, int D>
+template <typename T, int ELEM, int D, int NR>
 int launch(const Call& a, cudaStream_t st) {
-  constexpr int bytes = Layout<ELEM, D>::bytes;
-  const int ctas = ctas_of(a), rows = a.T * (a.Hq / a.cache.Hkv);
-  constexpr int id = (std::is_same_v<T, __half> ? 100 : 0) + ELEM * 10 + D;
-  if (rows <= 8) {
-    if (!allow_smem<1000 + id>(kv_attention_kernel<T, ELEM, D, 1>, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-    kv_attention_kernel<T, ELEM, D, 1><<<ctas, 32 * kWarps, bytes, st>>>(a);
-  } else {
-    if (!allow_smem<2000 + id>(kv_attention_kernel<T, ELEM, D, 2>, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-    kv_attention_kernel<T, ELEM, D, 2><<<ctas, 32 * kWarps, bytes, st>>>(a);
-  }
+  constexpr int bytes = Layout<ELEM, D, NR>::bytes;
+  constexpr int id = (std::is_same_v<T, __half> ? 10000 : 0) + ELEM * 1000 + D * 8 + NR;
+  const int ctas = ctas_of(a);
+  if (!allow_smem<id>(kv_attention_kernel<T, ELEM, D, NR>, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
+  kv_attention_kernel<T, ELEM, D, NR><<<ctas, 32 * kWarps, bytes, st>>>(a);
   if (int rc = check_launch("kv_attention")) return rc;
-  const dim3 grid(a.B * a.cache.Hkv * a.groups, (min(rows, kRows) + kWarps - 1) / kWarps);
+  const dim3 grid(a.B * a.cache.Hkv * a.groups, 2 * NR);
   launch_dependent(kv_combine_kernel<T, D>, grid, 32 * kWarps, 0, st, true, a, ctas);
   return check_launch("kv_attention");
 }
+template <typename T, int ELEM, int D>
+int launch_tiles(const Call& a, cudaStream_t st) {
+  return a.tiles == 1 ? launch<T, ELEM, D, 1>(a, st) : a.tiles == 2 ? launch<T, ELEM, D, 2>(a, st) : launch<T, ELEM, D, 4>(a, st);
+}
 template <typename T, int ELEM>
 int launch_depth(const Call& a, cudaStream_t st) {
-  return a.cache.D == 64 ? launch<T, ELEM, 64>(a, st) : launch<T, ELEM, 128>(a, st);
+  return a.cache.D == 64 ? launch_tiles<T, ELEM, 64>(a, st) : launch_tiles<T, ELEM, 128>(a, st);
 }
 template <typename T>
 int launch_elem(const Call& a, cudaStream_t st) {
@@ -584,9 +650,11 @@ long long plan(const mpsa_kv_attention_args* args, Call& a) {
   if (a.Hq % a.cache.Hkv) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: Hq must be a multiple of Hkv");
   if (a.B > 65535 || a.Hq > 65535 || a.T > 1024) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: at most 65535 sequences and 1024 query tokens");
   if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: sm_scale must be positive and finite");
-  a.groups = (a.T * (a.Hq / a.cache.Hkv) + kRows - 1) / kRows;
+  const int rows = a.T * (a.Hq / a.cache.Hkv);
+  a.tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  a.groups = (rows + 8 * a.tiles - 1) / (8 * a.tiles);
   if ((long long)a.B * a.cache.Hkv * a.groups > 0x7fffffffll) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: too many sequences and heads");
-  const long long slots = 2ll * ctas_of(a) * kRows;
+  const long long slots = 2ll * ctas_of(a) * 8 * a.tiles;
   a.part = static_cast<float*>(a.workspace);
   a.stat = reinterpret_cast<float2*>(a.part + slots * a.cache.D);
   return slots * (a.cache.D * 4 + 8);
