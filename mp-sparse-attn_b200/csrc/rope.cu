@@ -12,9 +12,12 @@ struct NormRope : mpsa_norm_rope_args {
   int heads_per_cta;            // norm 0 / 1: heads of one CTA, of the H[0] + H[1] in a row
 };
 
-__device__ __forceinline__ float weight_at(const void* w, int type, int i) {
-  return type == 2 ? static_cast<const float*>(w)[i]
-                   : type == 1 ? __half2float(static_cast<const __half*>(w)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+// 4 weights at i, a multiple of 4
+__device__ __forceinline__ void weights4(const void* w, int type, int i, float (&x)[4]) {
+  if (!w) x[0] = x[1] = x[2] = x[3] = 1.0f;
+  else if (type == 2) load4(static_cast<const float*>(w) + i, x);
+  else if (type == 1) load4(static_cast<const __half*>(w) + i, x);
+  else load4(static_cast<const __nv_bfloat16*>(w) + i, x);
 }
 
 // A lane holds 8 elements of a row as two runs of 4: where rotated pairs lie half the rotated width apart, 4 of each half, so that both
@@ -29,49 +32,54 @@ __device__ __forceinline__ Place place(int j, int rot, bool interleaved) {
   return {{4 * j, rot / 2 + 4 * j}, true};
 }
 
-// Cosines and sines of the lane's four pairs for token (b, l).
+// The table's rows for the axes of token (b, l); false: a position outside it.
+__device__ __forceinline__ bool positions_of(const NormRope& a, int b, int l, long long (&pos)[kMaxAxes]) {
+  if (!a.positions) {
+    pos[0] = l;
+    return l < a.table_rows;
+  }
+  bool there = true;
+  const long long at = b * a.pos_sb + (long long)l * a.axes;
+#pragma unroll
+  for (int i = 0; i < kMaxAxes; ++i)
+    if (i < a.axes) {
+      pos[i] = a.pos64 ? static_cast<const long long*>(a.positions)[at + i] : static_cast<const int*>(a.positions)[at + i];
+      there = there && pos[i] >= 0 && pos[i] < a.table_rows;
+    }
+  return there;
+}
+__device__ __forceinline__ long long row_of_pair(const NormRope& a, const long long (&pos)[kMaxAxes], int pair) {
+  long long row = pos[0];
+#pragma unroll
+  for (int x = 1; x < kMaxAxes; ++x)
+    if (x < a.axes && pair >= a.section_end[x - 1]) row = pos[x];
+  return row;
+}
+
+// Cosines and sines of a lane's four pairs for token (b, l).
 __device__ __forceinline__ void angles(const NormRope& a, int b, int l, int j, float (&c)[4], float (&s)[4]) {
   const float *cos = static_cast<const float*>(a.cos), *sin = static_cast<const float*>(a.sin);
   const int half = a.rot / 2;
-  bool there = true;
-  long long row[4];
-  if (!a.positions) {
-    row[0] = row[1] = row[2] = row[3] = l;
-    there = l < a.table_rows;
-  } else {
-    long long pos[kMaxAxes] = {};
-    const long long at = b * a.pos_sb + (long long)l * a.axes;
-#pragma unroll
-    for (int i = 0; i < kMaxAxes; ++i)
-      if (i < a.axes) {
-        pos[i] = a.pos64 ? static_cast<const long long*>(a.positions)[at + i] : static_cast<const int*>(a.positions)[at + i];
-        there = there && pos[i] >= 0 && pos[i] < a.table_rows;
-      }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      row[i] = pos[0];
-#pragma unroll
-      for (int x = 1; x < kMaxAxes; ++x)
-        if (x < a.axes && 4 * j + i >= a.section_end[x - 1]) row[i] = pos[x];
-    }
-  }
-  if (!there) {
+  long long pos[kMaxAxes] = {};
+  if (!positions_of(a, b, l, pos)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
   } else if (a.axes == 1) {
-    load4(cos + row[0] * half + 4 * j, c);
-    load4(sin + row[0] * half + 4 * j, s);
+    load4(cos + pos[0] * half + 4 * j, c);
+    load4(sin + pos[0] * half + 4 * j, s);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      c[i] = cos[row[i] * half + 4 * j + i];
-      s[i] = sin[row[i] * half + 4 * j + i];
+      const long long at = row_of_pair(a, pos, 4 * j + i) * half + 4 * j + i;
+      c[i] = cos[at];
+      s[i] = sin[at];
     }
   }
 }
 
-__device__ __forceinline__ void turn(float (&u)[4], float (&v)[4], const float (&c)[4], const float (&s)[4], bool interleaved) {
-  if (interleaved) {
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn(float (&u)[4], float (&v)[4], const float (&c)[4], const float (&s)[4]) {
+  if constexpr (INTERLEAVED) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float a = u[2 * i], b = u[2 * i + 1], d = v[2 * i], e = v[2 * i + 1];
@@ -97,117 +105,170 @@ __device__ __forceinline__ float squares(const float (&u)[4], const float (&v)[4
   return q;
 }
 
-// Norm of each head, or none: D/8 lanes hold a row; they keep the token's angles for all of the CTA's heads.
-template <typename T, int LANES>
+// Norm of each head, or none: D/8 lanes hold a row; they keep the token's angles for all of the CTA's heads, and the operand's weights.
+// kAhead rows are requested before the first is worked on.
+constexpr int kAhead = 4;
+template <typename T, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) norm_rope_heads_kernel(const __grid_constant__ NormRope a) {
   const int j = threadIdx.x % LANES;
   const long long n = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = n < (long long)a.B * a.L;
   const int b = live ? (int)(n / a.L) : 0, l = live ? (int)(n % a.L) : 0;
-  const Place p = place(j, a.cos ? a.rot : 0, a.interleaved);
-  float c[4], s[4], w[2][8];
+  const Place p = place(j, a.cos ? a.rot : 0, INTERLEAVED);
+  float c[4] = {1, 1, 1, 1}, s[4] = {};
   if (p.turned) angles(a, b, l, j, c, s);
 #pragma unroll
-  for (int o = 0; o < 2; ++o)
+  for (int o = 0; o < 2; ++o) {
+    const int before = o ? a.H[0] : 0;
+    const int first = max((int)blockIdx.y * a.heads_per_cta - before, 0), last = min(((int)blockIdx.y + 1) * a.heads_per_cta - before, a.H[o]);
+    if (first >= last) continue;
+    float w0[4], w1[4];
+    weights4(a.weight[o], a.w_dtype[o], p.at[0], w0);
+    weights4(a.weight[o], a.w_dtype[o], p.at[1], w1);
+    const long long xh = a.x_sh[o], yh = a.y_sh[o];
+    const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + first * xh);
+    T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + first * yh);
+    for (int h = first; h < last; h += kAhead) {
+      Raw4<T> r0[kAhead], r1[kAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[o][i] = a.weight[o] ? weight_at(a.weight[o], a.w_dtype[o], p.at[i / 4] + i % 4) : 1.0f;
-  const int first = blockIdx.y * a.heads_per_cta, last = min(first + a.heads_per_cta, a.H[0] + a.H[1]);
-#pragma unroll 2
-  for (int h = first; h < last; ++h) {
-    const int o = h >= a.H[0], head = o ? h - a.H[0] : h;
-    const T* x = static_cast<const T*>(o ? a.x[1] : a.x[0]) + (b * (o ? a.x_sb[1] : a.x_sb[0]) + head * (o ? a.x_sh[1] : a.x_sh[0]) + l * (o ? a.x_sl[1] : a.x_sl[0]));
-    T* y = static_cast<T*>(o ? a.y[1] : a.y[0]) + (b * (o ? a.y_sb[1] : a.y_sb[0]) + head * (o ? a.y_sh[1] : a.y_sh[0]) + l * (o ? a.y_sl[1] : a.y_sl[0]));
-    float u[4], v[4];
-    load4(x + p.at[0], u);
-    load4(x + p.at[1], v);
-    if (a.norm) {
-      float q = squares(u, v);
+      for (int k = 0; k < kAhead; ++k)
+        if (h + k < last) {
+          r0[k] = raw4(x + k * xh + p.at[0]);
+          r1[k] = raw4(x + k * xh + p.at[1]);
+        }
 #pragma unroll
-      for (int d = LANES / 2; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
-      const float r = 1.0f / sqrtf(q * (1.0f / (8 * LANES)) + a.eps);
+      for (int k = 0; k < kAhead; ++k) {
+        if (h + k >= last) break;
+        float u[4], v[4];
+        wide4(r0[k], u);
+        wide4(r1[k], v);
+        if (a.norm) {
+          float q = squares(u, v);
+#pragma unroll
+          for (int d = LANES / 2; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
+          const float r = rsqrtf(q * (1.0f / (8 * LANES)) + a.eps);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            u[i] *= r * w0[i];
+            v[i] *= r * w1[i];
+          }
+        }
+        if (p.turned) turn<INTERLEAVED>(u, v, c, s);
+        if (live) {
+          store4(y + k * yh + p.at[0], u);
+          store4(y + k * yh + p.at[1], v);
+        }
+      }
+      x += kAhead * xh;
+      y += kAhead * yh;
+    }
+  }
+}
+
+// Norm across the heads of a token: a CTA holds one token of one operand in registers, CHUNKS x 8 elements a thread, and takes tokens in
+// turn: the weights stay where they are.  A token's angles go through shared memory, with the partial sums (two buffers: one barrier a token).
+template <typename T, int LANES, int CHUNKS, bool INTERLEAVED>
+__global__ void __launch_bounds__(512) norm_rope_across_kernel(const __grid_constant__ NormRope a) {
+  __shared__ float part[2][16];
+  __shared__ __align__(16) float angle[2][2][4 * LANES];
+  const int o = blockIdx.y, H = a.H[o], half = a.rot / 2;
+  const int j = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES, warps = blockDim.x / 32;
+  const Place p = place(j, a.cos ? a.rot : 0, INTERLEAVED);
+  float w[CHUNKS][2][4];
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k) {
+    const int h = min(k * groups + group, H - 1);
+    weights4(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[0], w[k][0]);
+    weights4(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[1], w[k][1]);
+  }
+  const long long xh = groups * a.x_sh[o], yh = groups * a.y_sh[o];
+  int turnover = 0;
+  for (long long n = blockIdx.x; n < (long long)a.B * a.L; n += gridDim.x, turnover ^= 1) {
+    const int b = (int)(n / a.L), l = (int)(n % a.L);
+    const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + group * a.x_sh[o]);
+    T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + group * a.y_sh[o]);
+    Raw4<T> r0[CHUNKS], r1[CHUNKS];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k)
+      if (k * groups + group < H) {
+        r0[k] = raw4(x + k * xh + p.at[0]);
+        r1[k] = raw4(x + k * xh + p.at[1]);
+      }
+    if (a.cos)
+      for (int i = threadIdx.x; i < half; i += blockDim.x) {
+        long long pos[kMaxAxes] = {};
+        const bool there = positions_of(a, b, l, pos);
+        const long long at = there ? row_of_pair(a, pos, i) * half + i : 0;
+        angle[turnover][0][i] = there ? static_cast<const float*>(a.cos)[at] : __int_as_float(0x7fffffff);
+        angle[turnover][1][i] = there ? static_cast<const float*>(a.sin)[at] : __int_as_float(0x7fffffff);
+      }
+    float q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k)
+      if (k * groups + group < H) {
+        float u[4], v[4];
+        wide4(r0[k], u);
+        wide4(r1[k], v);
+        q += squares(u, v);
+      }
+#pragma unroll
+    for (int d = 16; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
+    if (threadIdx.x % 32 == 0) part[turnover][threadIdx.x / 32] = q;
+    __syncthreads();
+    q = threadIdx.x % 16 < warps ? part[turnover][threadIdx.x % 16] : 0.0f;
+#pragma unroll
+    for (int d = 8; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
+    const float r = rsqrtf(q / (float)(H * 8 * LANES) + a.eps);
+    float c[4] = {1, 1, 1, 1}, s[4] = {};
+    if (p.turned) {
+      load4(&angle[turnover][0][4 * j], c);
+      load4(&angle[turnover][1][4 * j], s);
+    }
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+      if (k * groups + group >= H) continue;
+      float u[4], v[4];
+      wide4(r0[k], u);
+      wide4(r1[k], v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u[i] = u[i] * r * (o ? w[1][i] : w[0][i]);
-        v[i] = v[i] * r * (o ? w[1][4 + i] : w[0][4 + i]);
+        u[i] *= r * w[k][0][i];
+        v[i] *= r * w[k][1][i];
       }
-    }
-    if (p.turned) turn(u, v, c, s, a.interleaved);
-    if (live) {
-      store4(y + p.at[0], u);
-      store4(y + p.at[1], v);
+      if (p.turned) turn<INTERLEAVED>(u, v, c, s);
+      store4(y + k * yh + p.at[0], u);
+      store4(y + k * yh + p.at[1], v);
     }
   }
 }
 
-// Norm across the heads of a token: a CTA holds one token of one operand in registers, CHUNKS x 8 elements a thread.
-template <typename T, int LANES, int CHUNKS>
-__global__ void norm_rope_across_kernel(const __grid_constant__ NormRope a) {
-  __shared__ float part[32];
-  const int o = blockIdx.y, H = a.H[o];
-  const int b = blockIdx.x / a.L, l = blockIdx.x % a.L;
-  const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o]);
-  T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o]);
-  const int j = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES;
-  const Place p = place(j, a.cos ? a.rot : 0, a.interleaved);
-  float u[CHUNKS][4], v[CHUNKS][4], q = 0.0f;
-#pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) {
-    const int h = k * groups + group;
-    if (h < H) {
-      load4(x + h * a.x_sh[o] + p.at[0], u[k]);
-      load4(x + h * a.x_sh[o] + p.at[1], v[k]);
-      q += squares(u[k], v[k]);
-    }
-  }
-  float c[4], s[4];
-  if (p.turned) angles(a, b, l, j, c, s);
-#pragma unroll
-  for (int d = 16; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = q;
-  __syncthreads();
-  q = 0.0f;
-  for (int i = 0; i < (int)(blockDim.x / 32); ++i) q += part[i];
-  const float r = 1.0f / sqrtf(q / (float)(H * 8 * LANES) + a.eps);
-#pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) {
-    const int h = k * groups + group;
-    if (h >= H) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u[k][i] *= r;
-      v[k][i] *= r;
-      if (a.weight[o]) {
-        u[k][i] *= weight_at(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[0] + i);
-        v[k][i] *= weight_at(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[1] + i);
-      }
-    }
-    if (p.turned) turn(u[k], v[k], c, s, a.interleaved);
-    store4(y + h * a.y_sh[o] + p.at[0], u[k]);
-    store4(y + h * a.y_sh[o] + p.at[1], v[k]);
-  }
-}
-
-template <typename T, int LANES>
+template <typename T, int LANES, bool INTERLEAVED>
 int launch(NormRope& a, cudaStream_t st) {
   const long long tokens = (long long)a.B * a.L;
   const int heads = a.H[0] + a.H[1];
   if (a.norm == 2) {
     const int most = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
-    const dim3 grid((unsigned)tokens, a.x[1] ? 2 : 1);
     const int chunks = (most * LANES + 511) / 512;                   // of a thread, with 512 threads at most
     const int per = (most + chunks - 1) / chunks;
     const int threads = (per * LANES + 31) / 32 * 32;
-    if (chunks == 1) norm_rope_across_kernel<T, LANES, 1><<<grid, threads, 0, st>>>(a);
-    else if (chunks == 2) norm_rope_across_kernel<T, LANES, 2><<<grid, threads, 0, st>>>(a);
-    else norm_rope_across_kernel<T, LANES, 4><<<grid, threads, 0, st>>>(a);
+    const long long resident = 2048 / threads * (long long)sm_count();
+    const dim3 grid((unsigned)(tokens < resident ? tokens : resident), a.x[1] ? 2 : 1);
+    if (chunks == 1) norm_rope_across_kernel<T, LANES, 1, INTERLEAVED><<<grid, threads, 0, st>>>(a);
+    else if (chunks == 2) norm_rope_across_kernel<T, LANES, 2, INTERLEAVED><<<grid, threads, 0, st>>>(a);
+    else norm_rope_across_kernel<T, LANES, 4, INTERLEAVED><<<grid, threads, 0, st>>>(a);
     return check_launch("norm_rope");
   }
   const long long groups = (tokens + kThreads / LANES - 1) / (kThreads / LANES);
   a.heads_per_cta = heads;                                           // split over CTAs where there are few tokens
-  while (a.heads_per_cta > 1 && groups * ((heads + a.heads_per_cta - 1) / a.heads_per_cta) < 8ll * sm_count()) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+  while (a.heads_per_cta > kAhead && groups * ((heads + a.heads_per_cta - 1) / a.heads_per_cta) < 8ll * sm_count()) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid((unsigned)groups, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
-  norm_rope_heads_kernel<T, LANES><<<grid, kThreads, 0, st>>>(a);
+  norm_rope_heads_kernel<T, LANES, INTERLEAVED><<<grid, kThreads, 0, st>>>(a);
   return check_launch("norm_rope");
+}
+template <typename T>
+int launch_depth(NormRope& a, cudaStream_t st) {
+  if (a.D == 64) return a.interleaved ? launch<T, 8, true>(a, st) : launch<T, 8, false>(a, st);
+  return a.interleaved ? launch<T, 16, true>(a, st) : launch<T, 16, false>(a, st);
 }
 
 }  // namespace
@@ -233,6 +294,7 @@ extern "C" int mpsa_norm_rope(const mpsa_norm_rope_args* args, void* stream) {
     if ((a.x_sb[o] | a.x_sh[o] | a.x_sl[o] | a.y_sb[o] | a.y_sh[o] | a.y_sl[o]) % 4 || (uintptr_t)a.x[o] % (4 * size) || (uintptr_t)a.y[o] % (4 * size))
       return set_error(MPSA_ERR_UNSUPPORTED, "norm_rope: bases and strides must be multiples of 4 elements");
     if (a.w_dtype[o] < 0 || a.w_dtype[o] > 2) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: weights must be bf16, fp16 or fp32");
+    if ((uintptr_t)a.weight[o] % 16) return set_error(MPSA_ERR_UNSUPPORTED, "norm_rope: weights must be 16-byte aligned");
   }
   if ((a.cos != nullptr) != (a.sin != nullptr)) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: cos and sin go together");
   if (a.cos) {
@@ -244,7 +306,5 @@ extern "C" int mpsa_norm_rope(const mpsa_norm_rope_args* args, void* stream) {
         return set_error(MPSA_ERR_BAD_ARG, "norm_rope: sections must ascend and end at rot / 2");
   }
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a.D == 64)
-    return a.in_dtype == 0 ? launch<__nv_bfloat16, 8>(a, st) : a.in_dtype == 1 ? launch<__half, 8>(a, st) : launch<float, 8>(a, st);
-  return a.in_dtype == 0 ? launch<__nv_bfloat16, 16>(a, st) : a.in_dtype == 1 ? launch<__half, 16>(a, st) : launch<float, 16>(a, st);
+  return a.in_dtype == 0 ? launch_depth<__nv_bfloat16>(a, st) : a.in_dtype == 1 ? launch_depth<__half>(a, st) : launch_depth<float>(a, st);
 }

@@ -11,21 +11,22 @@ namespace mpsa {
 
 enum Elem : int { E4M3 = 0, E5M2 = 1, E2M1 = 2 };
 
-// 4 neighbouring elements, 8 or 16 bytes at once
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xffff0000u);
-  x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xffff0000u);
+// 4 neighbouring elements, 8 or 16 bytes at once: as they are in memory, and in fp32
+template <typename T> struct Raw4 { uint2 u; };
+template <> struct Raw4<float> { float4 u; };
+template <typename T>
+__device__ __forceinline__ Raw4<T> raw4(const T* p) { return {*reinterpret_cast<const decltype(Raw4<T>::u)*>(p)}; }
+__device__ __forceinline__ void wide4(const Raw4<__nv_bfloat16>& r, float (&x)[4]) {
+  x[0] = __uint_as_float(r.u.x << 16); x[1] = __uint_as_float(r.u.x & 0xffff0000u);
+  x[2] = __uint_as_float(r.u.y << 16); x[3] = __uint_as_float(r.u.y & 0xffff0000u);
 }
-__device__ __forceinline__ void load4(const __half* p, float (&x)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+__device__ __forceinline__ void wide4(const Raw4<__half>& r, float (&x)[4]) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.u.y));
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
-__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
-  const float4 u = *reinterpret_cast<const float4*>(p);
-  x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-}
+__device__ __forceinline__ void wide4(const Raw4<float>& r, float (&x)[4]) { x[0] = r.u.x; x[1] = r.u.y; x[2] = r.u.z; x[3] = r.u.w; }
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&x)[4]) { wide4(raw4(p), x); }
 
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);

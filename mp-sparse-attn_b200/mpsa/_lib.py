@@ -106,7 +106,7 @@ class _LongWay:
     def attention(*_):
         return None
 
-    quant_pair = gemm = attention
+    quant_pair = gemm = kv_cache = norm_rope = kv_append = kv_read = kv_attention = attention
 
 
 def _module(name, path):
@@ -131,6 +131,8 @@ def native():
         mod = _module("mpsa._native", path if os.path.exists(path) else build.build_native())
         mod.init(*(ctypes.cast(getattr(lib, f), c_void_p).value for f in
                    ("mpsa_attention_workspace", "mpsa_attention", "mpsa_quant_pair", "mpsa_gemm_block_scaled")), torch.OutOfMemoryError)
+        mod.init_serving(*(ctypes.cast(getattr(lib, f), c_void_p).value for f in
+                           ("mpsa_norm_rope", "mpsa_kv_append", "mpsa_kv_read", "mpsa_kv_attention_workspace", "mpsa_kv_attention")))
     except Exception as e:                       # noqa: BLE001 (whatever kept it from being built or loaded)
         import warnings
         warnings.warn(f"mpsa: the native module for short calls is not available, they go through ctypes ({type(e).__name__}: {str(e)[:500]})", RuntimeWarning,

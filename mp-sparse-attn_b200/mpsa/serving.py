@@ -76,6 +76,14 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
     positions: int32 or int64, [L] or [B,L]; None: token l has position l.  With `sections` (R/2 split among up to four axes, in pairs)
     positions are [L,A] or [B,L,A], and pair i goes by the axis that its section belongs to.  A token with a position outside the table
     gets NaN in its rotated elements."""
+    r = None
+    if tensor_layout in ("HND", "NHD") and (rope is None or len(rope) == 2):
+        r = _lib.native().norm_rope(q, k, q_weight, k_weight, (2 if across_heads else 1) if norm else 0, eps, *((None, None) if rope is None else rope), positions, sections,
+                                    interleaved, tensor_layout == "HND")
+    if r is not None:
+        if r.__class__ is int:
+            _lib.check(r)
+        return r
     _require_cuda(q, k, q_weight, k_weight, positions)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         raise ValueError("norm_rope computes no gradient: call it under torch.no_grad()")
@@ -107,6 +115,9 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
             if w.device != q.device or w.dtype not in _IN_DTYPE or w.numel() != (H * D if across_heads else D) or \
                     tuple(w.shape) not in ((D,), (H, D), (H * D,)) or not w.is_contiguous():
                 raise ValueError("weights must be contiguous [D], or [H, D] or [H * D] across heads, on q's device")
+            if w.data_ptr() % 16:
+                w = w.clone()
+                keep.append(w)
             a.weight[i], a.w_dtype[i] = w.data_ptr(), _IN_DTYPE[w.dtype]
         outs.append(y)
         keep.append(x)
@@ -166,6 +177,9 @@ class KVCache:
     def __post_init__(self):
         if self.elem not in _ELEM:
             raise ValueError(f"unknown cache element {self.elem!r}")
+        self._c = _lib.native().kv_cache(self.k, self.k_scale, self.v, self.v_scale, _ELEM[self.elem])       # the argument block, as bytes
+        if self._c is not None:
+            return
         _require_cuda(self.k, self.v, self.k_scale, self.v_scale)
         if self.k.dim() != 4:
             raise ValueError("cache codes must be [pages, heads, page size, bytes]")
@@ -174,8 +188,8 @@ class KVCache:
         for t, n in ((self.k, row), (self.v, row), (self.k_scale, D // 32), (self.v_scale, D // 32)):
             if t.dtype is not torch.uint8 or t.shape != (pages, heads, page, n) or not t.is_contiguous() or t.device != self.k.device:
                 raise ValueError("cache buffers must be contiguous uint8 [pages, heads, page size, ...] on one device")
-        self._c = _Cache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), pages, page, heads, D,
-                         _ELEM[self.elem])
+        self._c = bytes(_Cache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), pages, page, heads, D,
+                               _ELEM[self.elem]))
 
     @property
     def num_kv_heads(self) -> int:
@@ -187,7 +201,10 @@ class KVCache:
 
     @property
     def head_dim(self) -> int:
-        return self._c.D
+        return self.k.shape[3] * (2 if self.elem == "e2m1" else 1)
+
+    def _block(self) -> _Cache:
+        return _Cache.from_buffer_copy(self._c)
 
 
 def kv_cache(num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64, elem: str = "e4m3", device="cuda") -> KVCache:
@@ -225,6 +242,10 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     is left out.  counts int32 [B]: only the first counts[b] tokens are written (a padded batch).  start int32 [B].
     A block's scale is the smallest power of two at which no element exceeds the type's largest value; a block with a NaN or an infinity
     reads back as NaN.  Pages written by one call must not be shared between its sequences."""
+    if tensor_layout in ("HND", "NHD"):
+        r = _lib.native().kv_append(cache._c, cache.k, k, v, page_table, start, counts, tensor_layout == "HND")
+        if r is not None:
+            return _lib.check(r)
     _require_cuda(k, v, page_table, start, counts)
     if k.dtype not in _IN_DTYPE or v.dtype != k.dtype:
         raise ValueError(f"unsupported input dtypes {k.dtype}, {v.dtype}")
@@ -238,7 +259,7 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     _table(page_table, B, dev)
     _index(start, "start", (B,), dev)
     _index(counts, "counts", (B,), dev, True)
-    a = _AppendArgs(cache._c, k.data_ptr(), v.data_ptr(), *ks, *vs, page_table.stride(0), page_table.data_ptr(), start.data_ptr(), _ptr(counts),
+    a = _AppendArgs(cache._block(), k.data_ptr(), v.data_ptr(), *ks, *vs, page_table.stride(0), page_table.data_ptr(), start.data_ptr(), _ptr(counts),
                     _IN_DTYPE[k.dtype], B, T, page_table.shape[1])
     _lib.check(_on_device(dev.index, _lib.load().mpsa_kv_append, ctypes.byref(a)))
 
@@ -248,6 +269,12 @@ def kv_cache_read(cache: KVCache, page_table: torch.Tensor, lengths: torch.Tenso
     """The cached keys and values of whole sequences in out_dtype (bf16, fp16, fp32): two tensors [B, Hkv, max_len, D], zero from lengths[b]
     on and where the table names no page.  max_len: all that the table can hold unless given.  For a prefill over a cached prefix
     (attention_forward takes them as k and v)."""
+    if max_len is not None and out_dtype in _OUT_DTYPE:
+        r = _lib.native().kv_read(cache._c, cache.k, page_table, lengths, max_len, _OUT_DTYPE[out_dtype])
+        if r is not None:
+            if r.__class__ is int:
+                _lib.check(r)
+            return r
     _require_cuda(page_table, lengths)
     dev = cache.k.device
     B = page_table.shape[0]
@@ -259,7 +286,7 @@ def kv_cache_read(cache: KVCache, page_table: torch.Tensor, lengths: torch.Tenso
     if n <= 0:
         raise ValueError("max_len must be positive")
     k, v = (torch.empty((B, cache.num_kv_heads, n, cache.head_dim), dtype=out_dtype, device=dev) for _ in range(2))
-    a = _ReadArgs(cache._c, k.data_ptr(), v.data_ptr(), page_table.stride(0), page_table.data_ptr(), lengths.data_ptr(), _OUT_DTYPE[out_dtype], B, n,
+    a = _ReadArgs(cache._block(), k.data_ptr(), v.data_ptr(), page_table.stride(0), page_table.data_ptr(), lengths.data_ptr(), _OUT_DTYPE[out_dtype], B, n,
                   page_table.shape[1])
     _lib.check(_on_device(dev.index, _lib.load().mpsa_kv_read, ctypes.byref(a)))
     return k, v
@@ -276,6 +303,13 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     mask: bool [T,T] or [B,T,T], True where query token i sees query token j - a tree of drafted tokens; None: every token sees those before
     it and itself.  Cached tokens before the query tokens are seen by all.  A row that sees nothing is zero.
     return_lse: also fp32 [B,Hq,T], log2 of the softmax denominators (-inf for a row that sees nothing), as attention_merge takes it."""
+    if tensor_layout in ("HND", "NHD"):
+        r = _lib.native().kv_attention(cache._c, cache.k, q, page_table, lengths, q_lens, mask,
+                                       cache.head_dim ** -0.5 if sm_scale is None else sm_scale, return_lse, tensor_layout == "HND")
+        if r is not None:
+            if r.__class__ is int:
+                _lib.check(r)
+            return r
     _require_cuda(q, page_table, lengths, q_lens, mask)
     dev = cache.k.device
     if q.dtype not in (torch.bfloat16, torch.float16):
@@ -298,7 +332,7 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     _, _, os = _bhld(out, tensor_layout)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
-    a = _AttentionArgs(cache._c, q.data_ptr(), out.data_ptr(), _ptr(lse), None, 0, *qs, *os, page_table.stride(0),
+    a = _AttentionArgs(cache._block(), q.data_ptr(), out.data_ptr(), _ptr(lse), None, 0, *qs, *os, page_table.stride(0),
                        0 if mask is None or mask.dim() == 2 else T * T, page_table.data_ptr(), lengths.data_ptr(), _ptr(q_lens), _ptr(mask),
                        _IN_DTYPE[q.dtype], B, T, Hq, page_table.shape[1], sm)
     lib = _lib.load()
