@@ -293,7 +293,7 @@ int mpsa_gemm_block_scaled_batched(const void* a, const void* a_scale, const voi
  * in fp32, rounded once.  Pair i is (y[i], y[i + rot/2]), or with interleaved (y[2i], y[2i + 1]); elements from `rot` on are not rotated.
  *   x, y       [B,H,L,D], element strides, innermost dense; strides multiples of 4, bases of 4 elements.  x[1] null: one operand.
  *              y may be x itself with the same strides.
- *   weight     null: no weight; 16-byte aligned.  w_dtype as in_dtype, each operand's own
+ *   weight     null: no weight; 16-byte aligned.  w_dtype: in_dtype or 2 (fp32), the same for both
  *   cos, sin   fp32 [table_rows, rot/2], 16-byte aligned; null: no rotation (rot is then ignored)
  *   positions  int32 (pos64 0) or int64 (1) [B or 1, L, axes], batch stride pos_sb; null: token l has position l (one axis).  With
  *              several axes pair i goes by the axis a with section_end[a-1] <= i < section_end[a].

@@ -48,29 +48,28 @@ __device__ __forceinline__ int length_of(const Call& a, int b) {
 __device__ __forceinline__ int queries_of(const Call& a, int b, int len) { return min(a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T, len); }
 __device__ __forceinline__ int steps_of(int len) { return max(1, (len + kStep - 1) / kStep); }    // (an empty sequence: one, which writes its zeros)
 
-// The steps of all units, and how many a CTA of `ctas` takes.  By a whole warp.
-__device__ long long share_of(const Call& a, int ctas, int lane) {
-  long long sum = 0;
-  for (int b = lane; b < a.B; b += 32) sum += steps_of(length_of(a, b));
-#pragma unroll
-  for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  sum *= a.cache.Hkv * a.groups;
-  return max((sum + ctas - 1) / ctas, (long long)kMinShare);
-}
-
-// The sequence that step `at` of all steps belongs to (a.B: beyond the last), and where that sequence's steps begin.
-__device__ int sequence_at(const Call& a, long long at, long long& begin, int lane) {
-  const int units = a.cache.Hkv * a.groups;
+// How many steps of all units a CTA takes (`share`), the sequence that step cta * share belongs to (returned; a.B: beyond the last) and where
+// that sequence's steps begin.  By a whole warp; plan() has seen to it that the steps of all units fit 32 bits.
+__device__ int locate(const Call& a, uint32_t ctas, uint32_t cta, uint32_t& share, uint32_t& begin, int lane) {
+  const uint32_t units = a.cache.Hkv * a.groups;
+  const uint32_t mine = lane < a.B ? steps_of(length_of(a, lane)) * units : 0;       // the first 32 sequences: read once
+  uint32_t sum = mine;
+  for (int b = lane + 32; b < a.B; b += 32) sum += steps_of(length_of(a, b)) * units;
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  share = max((sum + ctas - 1) / ctas, (uint32_t)kMinShare);
+  const unsigned long long want = (unsigned long long)cta * share;
   begin = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const long long n = b0 + lane < a.B ? (long long)steps_of(length_of(a, b0 + lane)) * units : 0;
-    long long up = n;
+  if (want >= sum) return a.B;
+  const uint32_t at = (uint32_t)want;
+  for (int b0 = 0;; b0 += 32) {
+    const uint32_t n = b0 == 0 ? mine : b0 + lane < a.B ? steps_of(length_of(a, b0 + lane)) * units : 0;
+    uint32_t up = n;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const long long v = __shfl_up_sync(0xffffffffu, up, d);
+      const uint32_t v = __shfl_up_sync(0xffffffffu, up, d);
       if (lane >= d) up += v;
     }
-    const unsigned beyond = __ballot_sync(0xffffffffu, b0 + lane < a.B && begin + up > at);
+    const unsigned beyond = __ballot_sync(0xffffffffu, begin + up > at);
     if (beyond) {
       const int l = __ffs(beyond) - 1;
       begin += __shfl_sync(0xffffffffu, up - n, l);
@@ -78,14 +77,12 @@ __device__ int sequence_at(const Call& a, long long at, long long& begin, int la
     }
     begin += __shfl_sync(0xffffffffu, up, 31);
   }
-  return a.B;
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {       // zeros where it is not
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -139,15 +136,8 @@ __device__ __forceinline__ void k_fragments(uint32_t p, uint32_t (&f)[ELEM == E2
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const uint32_t v = w[2 * i + x];                 // keys g + 8x
-      if constexpr (ELEM == E2M1) {
-        f[2 * i][x] = bits(elem_pair<ELEM>(v));
-        f[2 * i][2 + x] = bits(elem_pair<ELEM>(v >> 8));
-        f[2 * i + 1][x] = bits(elem_pair<ELEM>(v >> 16));
-        f[2 * i + 1][2 + x] = bits(elem_pair<ELEM>(v >> 24));
-      } else {
-        f[i][x] = bits(elem_pair<ELEM>(v));
-        f[i][2 + x] = bits(elem_pair<ELEM>(v >> 16));
-      }
+      if constexpr (ELEM == E2M1) elem_quads(v, f[2 * i][x], f[2 * i][2 + x], f[2 * i + 1][x], f[2 * i + 1][2 + x]);
+      else elem_two<ELEM>(v, f[i][x], f[i][2 + x]);
     }
 }
 
@@ -162,15 +152,14 @@ __device__ __forceinline__ void v_fragments(uint32_t p, uint32_t (&f)[ELEM == E2
     for (int x = 0; x < 2; ++x) {
       const uint32_t v = w[2 * i + x];                 // keys 8x + 2t (lower half) and 8x + 2t + 1
       if constexpr (ELEM == E2M1) {
-        const uint32_t a = bits(elem_pair<ELEM>(v)), b = bits(elem_pair<ELEM>(v >> 8)), c = bits(elem_pair<ELEM>(v >> 16)), d = bits(elem_pair<ELEM>(v >> 24));
+        uint32_t a, b, c, d;
+        elem_quads(v, a, b, c, d);
         f[2 * i][2 * x] = __byte_perm(a, c, 0x5410);
         f[2 * i][2 * x + 1] = __byte_perm(a, c, 0x7632);
         f[2 * i + 1][2 * x] = __byte_perm(b, d, 0x5410);
         f[2 * i + 1][2 * x + 1] = __byte_perm(b, d, 0x7632);
       } else {
-        const uint32_t u = __byte_perm(v, 0, 0x3120);
-        f[i][2 * x] = bits(elem_pair<ELEM>(u));
-        f[i][2 * x + 1] = bits(elem_pair<ELEM>(u >> 16));
+        elem_two<ELEM>(__byte_perm(v, 0, 0x3120), f[i][2 * x], f[i][2 * x + 1]);
       }
     }
 }
@@ -193,15 +182,14 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
   const uint32_t mat = (lane & 15) * Y::row + ((lane >> 4) ^ Y::swap(lane & 15)) * 16;  // this lane's row address for ldmatrix
 
   grid_dependents_go();
-  const long long share = share_of(a, gridDim.x, lane);
-  long long at = blockIdx.x * share;
-  const long long stop = at + share;
-  long long begin;
-  int b = sequence_at(a, at, begin, lane);
+  uint32_t share, begin;
+  int b = locate(a, gridDim.x, blockIdx.x, share, begin, lane);
+  uint32_t at = blockIdx.x * share;
+  const uint32_t stop = at + min(share, ~at);
   for (bool again = false; b < a.B && at < stop; again = true) {
     const int len = length_of(a, b), steps = steps_of(len);
-    const long long off = at - begin;
-    const int u = (int)(off / steps), s0 = (int)(off % steps), s1 = (int)min((long long)steps, s0 + (stop - at));
+    const uint32_t off = at - begin;
+    const int u = off / (uint32_t)steps, s0 = off - u * (uint32_t)steps, s1 = min((uint32_t)steps, s0 + (stop - at));
     const int h = u / a.groups, row0 = u % a.groups * Y::rows;
     const int ql = queries_of(a, b, len), first = len - ql;
     const int* const table = a.page_table + b * a.table_sb;
@@ -551,8 +539,8 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
       }
     }
     at += s1 - s0;
-    if (at >= begin + (long long)steps * units) {
-      begin += (long long)steps * units;
+    if (at - begin >= (uint32_t)steps * units) {
+      begin += (uint32_t)steps * units;
       ++b;
     }
   }
@@ -564,35 +552,46 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, units = a.cache.Hkv * a.groups;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
   const int rows = 8 * a.tiles, r = blockIdx.y * kWarps + warp, G = a.Hq / a.cache.Hkv, row = u % a.groups * rows + r;
-  const long long share = share_of(a, ctas, lane);
-  long long begin = 0;
-  for (int i = lane; i < b; i += 32) begin += (long long)steps_of(length_of(a, i)) * units;
-#pragma unroll
-  for (int d = 16; d; d /= 2) begin += __shfl_xor_sync(0xffffffffu, begin, d);
+  uint32_t share, begin;
+  locate(a, ctas, 0, share, begin, lane);
+  begin = 0;
+  for (int i = lane; i < b; i += 32) begin += steps_of(length_of(a, i)) * units;
+  begin = __reduce_add_sync(0xffffffffu, begin);
   const int len = length_of(a, b), steps = steps_of(len), ql = queries_of(a, b, len);
-  begin += (long long)u * steps;
-  const long long c0 = begin / share, c1 = (begin + steps - 1) / share;
+  begin += u * steps;
+  const int c0 = begin / share, parts = (begin + steps - 1) / share - c0 + 1;
   grid_dependency_wait();                             // (by everybody: what follows on the stream counts on it)
-  if (c0 == c1 || row >= a.T * G) return;
-  float top = -INFINITY, sum = 0.0f;
-  for (long long i = c0; i <= c1; ++i) top = fmaxf(top, a.stat[(2 * i + (i == c0)) * rows + r].x);
+  if (parts == 1 || row >= a.T * G) return;
+  // part i lies in slot 2 (c0 + i), the first one in 2 c0 + 1: a lane takes one of 32 parts' statistics, and then all add up the rows
+  auto slot = [&](int i) { return (long long)(2 * (c0 + i) + (i == 0)) * rows + r; };
+  const float2 nothing = make_float2(-INFINITY, 0.0f), first = lane < parts ? a.stat[slot(lane)] : nothing;
+  float top = first.x, sum = 0.0f;
+  for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, a.stat[slot(i)].x);
+#pragma unroll
+  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   const float ref = top == -INFINITY ? 0.0f : top;
   constexpr int N = D / 32;
   float v[N] = {};
-#pragma unroll 4
-  for (long long i = c0; i <= c1; ++i) {
-    const long long at = (2 * i + (i == c0)) * rows + r;
-    const float2 st = a.stat[at];
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const float2 st = i0 == 0 ? first : i0 + lane < parts ? a.stat[slot(i0 + lane)] : nothing;
     const float f = exp2_fast(st.x - ref);
     sum += f * st.y;
-    if constexpr (N == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part + at * D + 4 * lane);
-      v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(a.part + at * D + 2 * lane);
-      v[0] += f * x.x; v[1] += f * x.y;
+    const int n = min(parts - i0, 32);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* const p = a.part + slot(i0 + i) * D + N * lane;
+      if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] += w * x.x; v[1] += w * x.y; v[2] += w * x.z; v[3] += w * x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] += w * x.x; v[1] += w * x.y;
+      }
     }
   }
+#pragma unroll
+  for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const int tok = row / G, hq = u / a.groups * G + row % G;
   const bool none = sum == 0.0f || tok >= ql;
   const float f = none ? 0.0f : 1.0f / sum;
@@ -653,7 +652,8 @@ long long plan(const mpsa_kv_attention_args* args, Call& a) {
   const int rows = a.T * (a.Hq / a.cache.Hkv);
   a.tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
   a.groups = (rows + 8 * a.tiles - 1) / (8 * a.tiles);
-  if ((long long)a.B * a.cache.Hkv * a.groups > 0x7fffffffll) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: too many sequences and heads");
+  const double most = (double)a.B * a.cache.Hkv * a.groups * (((double)a.max_pages * a.cache.page_size) / kStep + 1);
+  if (most > 4e9) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: sequences x heads x page table too large (%.1e steps of %d keys, at most 4e9)", most, kStep);
   const long long slots = 2ll * ctas_of(a) * 8 * a.tiles;
   a.part = static_cast<float*>(a.workspace);
   a.stat = reinterpret_cast<float2*>(a.part + slots * a.cache.D);

@@ -339,7 +339,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const int64_t D = z[3], most = c.norm == 2 ? z[h] * D : D;
       const bool shaped = w[i]->dim() == 1 ? w[i]->size(0) == most : w[i]->dim() == 2 && c.norm == 2 && w[i]->size(0) == z[h] && w[i]->size(1) == D;
       c.w_dtype[i] = any_dtype(*w[i]);
-      if (!shaped || c.w_dtype[i] < 0 || reinterpret_cast<uintptr_t>(w[i]->data_ptr()) % 16 || !w[i]->is_contiguous() || w[i]->get_device() != device || (grad && w[i]->requires_grad())) Py_RETURN_NONE;
+      if (!shaped || (c.w_dtype[i] != 2 && c.w_dtype[i] != c.in_dtype) || (i && w[0] && c.w_dtype[0] != c.w_dtype[1]) || reinterpret_cast<uintptr_t>(w[i]->data_ptr()) % 16 || !w[i]->is_contiguous() || w[i]->get_device() != device || (grad && w[i]->requires_grad())) Py_RETURN_NONE;
       c.weight[i] = w[i]->data_ptr();
     }
     c.B = (int)x[0]->size(0); c.L = (int)x[0]->size(l); c.D = (int)x[0]->size(3);

@@ -13,11 +13,10 @@ struct NormRope : mpsa_norm_rope_args {
 };
 
 // 4 weights at i, a multiple of 4
-__device__ __forceinline__ void weights4(const void* w, int type, int i, float (&x)[4]) {
-  if (!w) x[0] = x[1] = x[2] = x[3] = 1.0f;
-  else if (type == 2) load4(static_cast<const float*>(w) + i, x);
-  else if (type == 1) load4(static_cast<const __half*>(w) + i, x);
-  else load4(static_cast<const __nv_bfloat16*>(w) + i, x);
+template <typename W>
+__device__ __forceinline__ void weights4(const void* w, int i, float (&x)[4]) {
+  if (w) load4(static_cast<const W*>(w) + i, x);
+  else x[0] = x[1] = x[2] = x[3] = 1.0f;
 }
 
 // A lane holds 8 elements of a row as two runs of 4: where rotated pairs lie half the rotated width apart, 4 of each half, so that both
@@ -108,8 +107,8 @@ __device__ __forceinline__ float squares(const float (&u)[4], const float (&v)[4
 // Norm of each head, or none: D/8 lanes hold a row; they keep the token's angles for all of the CTA's heads, and the operand's weights.
 // kAhead rows are requested before the first is worked on.
 constexpr int kAhead = 4;
-template <typename T, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) norm_rope_heads_kernel(const __grid_constant__ NormRope a) {
+template <typename T, typename W, int LANES, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads, 4) norm_rope_heads_kernel(const __grid_constant__ NormRope a) {
   const int j = threadIdx.x % LANES;
   const long long n = (long long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool live = n < (long long)a.B * a.L;
@@ -123,152 +122,152 @@ __global__ void __launch_bounds__(kThreads) norm_rope_heads_kernel(const __grid_
     const int first = max((int)blockIdx.y * a.heads_per_cta - before, 0), last = min(((int)blockIdx.y + 1) * a.heads_per_cta - before, a.H[o]);
     if (first >= last) continue;
     float w0[4], w1[4];
-    weights4(a.weight[o], a.w_dtype[o], p.at[0], w0);
-    weights4(a.weight[o], a.w_dtype[o], p.at[1], w1);
+    weights4<W>(a.weight[o], p.at[0], w0);
+    weights4<W>(a.weight[o], p.at[1], w1);
     const long long xh = a.x_sh[o], yh = a.y_sh[o];
     const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + first * xh);
     T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + first * yh);
     for (int h = first; h < last; h += kAhead) {
-      Raw4<T> r0[kAhead], r1[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (h + k < last) {
-          r0[k] = raw4(x + k * xh + p.at[0]);
-          r1[k] = raw4(x + k * xh + p.at[1]);
-        }
+      Raw4<T> r[kAhead][2];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (h + k >= last) break;
+        r[k][0] = raw4(x + p.at[0]);
+        r[k][1] = raw4(x + p.at[1]);
+        if (h + k + 1 < last) x += xh;                               // (the last row again, behind the last)
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
         float u[4], v[4];
-        wide4(r0[k], u);
-        wide4(r1[k], v);
+        wide4(r[k][0], u);
+        wide4(r[k][1], v);
         if (a.norm) {
           float q = squares(u, v);
 #pragma unroll
           for (int d = LANES / 2; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
-          const float r = rsqrtf(q * (1.0f / (8 * LANES)) + a.eps);
+          const float n = rsqrtf(q * (1.0f / (8 * LANES)) + a.eps);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            u[i] *= r * w0[i];
-            v[i] *= r * w1[i];
+            u[i] *= n * w0[i];
+            v[i] *= n * w1[i];
           }
         }
         if (p.turned) turn<INTERLEAVED>(u, v, c, s);
-        if (live) {
-          store4(y + k * yh + p.at[0], u);
-          store4(y + k * yh + p.at[1], v);
+        if (live && h + k < last) {
+          store4(y + p.at[0], u);
+          store4(y + p.at[1], v);
+          y += yh;
         }
       }
-      x += kAhead * xh;
-      y += kAhead * yh;
     }
   }
 }
 
-// Norm across the heads of a token: a CTA holds one token of one operand in registers, CHUNKS x 8 elements a thread, and takes tokens in
-// turn: the weights stay where they are.  A token's angles go through shared memory, with the partial sums (two buffers: one barrier a token).
-template <typename T, int LANES, int CHUNKS, bool INTERLEAVED>
+// Norm across the heads of a token: a CTA takes one token of one operand, up to kChunks x 8 elements a thread, all in registers between the
+// sum and the rest.  Few threads a token and many CTAs an SM: the others' loads run under one's barrier.
+constexpr int kChunks = 8;
+template <typename T, typename W, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(512) norm_rope_across_kernel(const __grid_constant__ NormRope a) {
-  __shared__ float part[2][16];
-  __shared__ __align__(16) float angle[2][2][4 * LANES];
-  const int o = blockIdx.y, H = a.H[o], half = a.rot / 2;
+  __shared__ float part[16];
+  __shared__ __align__(16) float angle[2][4 * LANES];
+  const int o = blockIdx.y, H = a.H[o];
+  const int b = blockIdx.x / a.L, l = blockIdx.x % a.L;
   const int j = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES, warps = blockDim.x / 32;
   const Place p = place(j, a.cos ? a.rot : 0, INTERLEAVED);
-  float w[CHUNKS][2][4];
-#pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) {
-    const int h = min(k * groups + group, H - 1);
-    weights4(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[0], w[k][0]);
-    weights4(a.weight[o], a.w_dtype[o], h * 8 * LANES + p.at[1], w[k][1]);
-  }
+  const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + group * a.x_sh[o]);
+  T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + group * a.y_sh[o]);
   const long long xh = groups * a.x_sh[o], yh = groups * a.y_sh[o];
-  int turnover = 0;
-  for (long long n = blockIdx.x; n < (long long)a.B * a.L; n += gridDim.x, turnover ^= 1) {
-    const int b = (int)(n / a.L), l = (int)(n % a.L);
-    const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + group * a.x_sh[o]);
-    T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + group * a.y_sh[o]);
-    Raw4<T> r0[CHUNKS], r1[CHUNKS];
+  Raw4<T> r0[kChunks], r1[kChunks];
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k)
-      if (k * groups + group < H) {
-        r0[k] = raw4(x + k * xh + p.at[0]);
-        r1[k] = raw4(x + k * xh + p.at[1]);
-      }
-    if (a.cos)
-      for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        long long pos[kMaxAxes] = {};
-        const bool there = positions_of(a, b, l, pos);
-        const long long at = there ? row_of_pair(a, pos, i) * half + i : 0;
-        angle[turnover][0][i] = there ? static_cast<const float*>(a.cos)[at] : __int_as_float(0x7fffffff);
-        angle[turnover][1][i] = there ? static_cast<const float*>(a.sin)[at] : __int_as_float(0x7fffffff);
-      }
-    float q = 0.0f;
-#pragma unroll
-    for (int k = 0; k < CHUNKS; ++k)
-      if (k * groups + group < H) {
-        float u[4], v[4];
-        wide4(r0[k], u);
-        wide4(r1[k], v);
-        q += squares(u, v);
-      }
-#pragma unroll
-    for (int d = 16; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
-    if (threadIdx.x % 32 == 0) part[turnover][threadIdx.x / 32] = q;
-    __syncthreads();
-    q = threadIdx.x % 16 < warps ? part[turnover][threadIdx.x % 16] : 0.0f;
-#pragma unroll
-    for (int d = 8; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
-    const float r = rsqrtf(q / (float)(H * 8 * LANES) + a.eps);
-    float c[4] = {1, 1, 1, 1}, s[4] = {};
-    if (p.turned) {
-      load4(&angle[turnover][0][4 * j], c);
-      load4(&angle[turnover][1][4 * j], s);
+  for (int k = 0; k < kChunks; ++k) {
+    r0[k] = {}, r1[k] = {};
+    if (k * groups + group < H) {
+      r0[k] = raw4(x + p.at[0]);
+      r1[k] = raw4(x + p.at[1]);
     }
-#pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      if (k * groups + group >= H) continue;
-      float u[4], v[4];
-      wide4(r0[k], u);
-      wide4(r1[k], v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u[i] *= r * w[k][0][i];
-        v[i] *= r * w[k][1][i];
-      }
-      if (p.turned) turn<INTERLEAVED>(u, v, c, s);
-      store4(y + k * yh + p.at[0], u);
-      store4(y + k * yh + p.at[1], v);
+    x += xh;
+  }
+  if (a.cos) {
+    const int half = a.rot / 2;
+    long long pos[kMaxAxes] = {};
+    const bool there = positions_of(a, b, l, pos);
+    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+      const long long at = there ? row_of_pair(a, pos, i) * half + i : 0;
+      angle[0][i] = there ? static_cast<const float*>(a.cos)[at] : __int_as_float(0x7fffffff);
+      angle[1][i] = there ? static_cast<const float*>(a.sin)[at] : __int_as_float(0x7fffffff);
     }
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    float u[4], v[4];
+    wide4(r0[k], u);
+    wide4(r1[k], v);
+    q += squares(u, v);
+  }
+#pragma unroll
+  for (int d = 16; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = q;
+  __syncthreads();
+  q = (int)(threadIdx.x % 16) < warps ? part[threadIdx.x % 16] : 0.0f;
+#pragma unroll
+  for (int d = 8; d; d /= 2) q += __shfl_xor_sync(0xffffffffu, q, d);
+  const float r = rsqrtf(q / (float)(H * 8 * LANES) + a.eps);
+  float c[4] = {1, 1, 1, 1}, s[4] = {};
+  if (p.turned) {
+    load4(&angle[0][4 * j], c);
+    load4(&angle[1][4 * j], s);
+  }
+  const W* wp = static_cast<const W*>(a.weight[o]) + group * 8 * LANES;
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    if (k * groups + group >= H) return;
+    float u[4], v[4], w0[4] = {1, 1, 1, 1}, w1[4] = {1, 1, 1, 1};
+    if (a.weight[o]) {
+      load4(wp + p.at[0], w0);
+      load4(wp + p.at[1], w1);
+      wp += groups * 8 * LANES;
+    }
+    wide4(r0[k], u);
+    wide4(r1[k], v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] *= r * w0[i];
+      v[i] *= r * w1[i];
+    }
+    if (p.turned) turn<INTERLEAVED>(u, v, c, s);
+    store4(y + p.at[0], u);
+    store4(y + p.at[1], v);
+    y += yh;
   }
 }
 
-template <typename T, int LANES, bool INTERLEAVED>
+template <typename T, typename W, int LANES, bool INTERLEAVED>
 int launch(NormRope& a, cudaStream_t st) {
   const long long tokens = (long long)a.B * a.L;
   const int heads = a.H[0] + a.H[1];
   if (a.norm == 2) {
     const int most = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
-    const int chunks = (most * LANES + 511) / 512;                   // of a thread, with 512 threads at most
-    const int per = (most + chunks - 1) / chunks;
-    const int threads = (per * LANES + 31) / 32 * 32;
-    const long long resident = 2048 / threads * (long long)sm_count();
-    const dim3 grid((unsigned)(tokens < resident ? tokens : resident), a.x[1] ? 2 : 1);
-    if (chunks == 1) norm_rope_across_kernel<T, LANES, 1, INTERLEAVED><<<grid, threads, 0, st>>>(a);
-    else if (chunks == 2) norm_rope_across_kernel<T, LANES, 2, INTERLEAVED><<<grid, threads, 0, st>>>(a);
-    else norm_rope_across_kernel<T, LANES, 4, INTERLEAVED><<<grid, threads, 0, st>>>(a);
+    const int threads = (most * LANES + 32 * kChunks - 1) / (32 * kChunks) * 32;
+    norm_rope_across_kernel<T, W, LANES, INTERLEAVED><<<dim3((unsigned)tokens, a.x[1] ? 2 : 1), threads, 0, st>>>(a);
     return check_launch("norm_rope");
   }
   const long long groups = (tokens + kThreads / LANES - 1) / (kThreads / LANES);
   a.heads_per_cta = heads;                                           // split over CTAs where there are few tokens
   while (a.heads_per_cta > kAhead && groups * ((heads + a.heads_per_cta - 1) / a.heads_per_cta) < 8ll * sm_count()) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid((unsigned)groups, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
-  norm_rope_heads_kernel<T, LANES, INTERLEAVED><<<grid, kThreads, 0, st>>>(a);
+  norm_rope_heads_kernel<T, W, LANES, INTERLEAVED><<<grid, kThreads, 0, st>>>(a);
   return check_launch("norm_rope");
 }
-template <typename T>
+template <typename T, typename W>
 int launch_depth(NormRope& a, cudaStream_t st) {
-  if (a.D == 64) return a.interleaved ? launch<T, 8, true>(a, st) : launch<T, 8, false>(a, st);
-  return a.interleaved ? launch<T, 16, true>(a, st) : launch<T, 16, false>(a, st);
+  if (a.D == 64) return a.interleaved ? launch<T, W, 8, true>(a, st) : launch<T, W, 8, false>(a, st);
+  return a.interleaved ? launch<T, W, 16, true>(a, st) : launch<T, W, 16, false>(a, st);
+}
+template <typename T>
+int launch_weights(NormRope& a, cudaStream_t st) {
+  for (int o = 0; o < 2; ++o)
+    if (a.weight[o] && a.w_dtype[o] == 2) return launch_depth<T, float>(a, st);
+  return launch_depth<T, T>(a, st);
 }
 
 }  // namespace
@@ -293,9 +292,10 @@ extern "C" int mpsa_norm_rope(const mpsa_norm_rope_args* args, void* stream) {
   for (int o = 0; o < (a.x[1] ? 2 : 1); ++o) {
     if ((a.x_sb[o] | a.x_sh[o] | a.x_sl[o] | a.y_sb[o] | a.y_sh[o] | a.y_sl[o]) % 4 || (uintptr_t)a.x[o] % (4 * size) || (uintptr_t)a.y[o] % (4 * size))
       return set_error(MPSA_ERR_UNSUPPORTED, "norm_rope: bases and strides must be multiples of 4 elements");
-    if (a.w_dtype[o] < 0 || a.w_dtype[o] > 2) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: weights must be bf16, fp16 or fp32");
+    if (a.weight[o] && a.w_dtype[o] != 2 && a.w_dtype[o] != a.in_dtype) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: weights must be fp32 or of the inputs' type");
     if ((uintptr_t)a.weight[o] % 16) return set_error(MPSA_ERR_UNSUPPORTED, "norm_rope: weights must be 16-byte aligned");
   }
+  if (a.weight[0] && a.weight[1] && a.x[1] && a.w_dtype[0] != a.w_dtype[1]) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: the weights must have one type");
   if ((a.cos != nullptr) != (a.sin != nullptr)) return set_error(MPSA_ERR_BAD_ARG, "norm_rope: cos and sin go together");
   if (a.cos) {
     if (a.rot <= 0 || a.rot % 8 || a.rot > a.D) return set_error(MPSA_ERR_UNSUPPORTED, "norm_rope: rot must be a multiple of 8, at most D");
@@ -306,5 +306,5 @@ extern "C" int mpsa_norm_rope(const mpsa_norm_rope_args* args, void* stream) {
         return set_error(MPSA_ERR_BAD_ARG, "norm_rope: sections must ascend and end at rot / 2");
   }
   const cudaStream_t st = (cudaStream_t)stream;
-  return a.in_dtype == 0 ? launch_depth<__nv_bfloat16>(a, st) : a.in_dtype == 1 ? launch_depth<__half>(a, st) : launch_depth<float>(a, st);
+  return a.in_dtype == 0 ? launch_weights<__nv_bfloat16>(a, st) : a.in_dtype == 1 ? launch_weights<__half>(a, st) : launch_weights<float>(a, st);
 }

@@ -51,18 +51,16 @@ __device__ __forceinline__ int page_of(const int* table, int entry, int max_page
 
 constexpr __host__ __device__ int code_bytes(int elem, int D) { return elem == E2M1 ? D / 2 : D; }
 
-// What two codes stand for, in units of the block's scale.
+// What a word of codes stands for in units of the block's scale, as fp16 pairs (exact): four 8-bit codes, or eight 4-bit ones.
 template <int ELEM>
-__device__ __forceinline__ __half2 elem_pair(uint32_t two) {          // 16 bits of two 8-bit codes, or 8 bits of two 4-bit ones
-  uint32_t r;
-  if constexpr (ELEM == E2M1) {
-    asm("{\n.reg .b8 h;\ncvt.u8.u32 h, %1;\ncvt.rn.f16x2.e2m1x2 %0, h;\n}" : "=r"(r) : "r"(two));
-  } else {
-    const unsigned short s = (unsigned short)two;
-    if constexpr (ELEM == E4M3) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(s));
-    else asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(r) : "h"(s));
-  }
-  return *reinterpret_cast<const __half2*>(&r);
+__device__ __forceinline__ void elem_two(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (ELEM == E4M3) asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}" : "=r"(a), "=r"(b) : "r"(w));
+  else asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e5m2x2 %0, x;\ncvt.rn.f16x2.e5m2x2 %1, y;\n}" : "=r"(a), "=r"(b) : "r"(w));
+}
+__device__ __forceinline__ void elem_quads(uint32_t w, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm("{\n.reg .b8 x, y, z, u;\nmov.b32 {x, y, z, u}, %4;\ncvt.rn.f16x2.e2m1x2 %0, x;\ncvt.rn.f16x2.e2m1x2 %1, y;\ncvt.rn.f16x2.e2m1x2 %2, z;\n"
+      "cvt.rn.f16x2.e2m1x2 %3, u;\n}"
+      : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(w));
 }
 
 // 2^(code - 127); 255 is NaN, and 0 (which mpsa_kv_append never writes) counts as zero

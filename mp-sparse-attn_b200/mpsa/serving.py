@@ -115,9 +115,11 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
             if w.device != q.device or w.dtype not in _IN_DTYPE or w.numel() != (H * D if across_heads else D) or \
                     tuple(w.shape) not in ((D,), (H, D), (H * D,)) or not w.is_contiguous():
                 raise ValueError("weights must be contiguous [D], or [H, D] or [H * D] across heads, on q's device")
+            if any(u is not None and u.dtype != q.dtype for u in (q_weight, k_weight)):
+                w = w.float()                          # (the kernels take the weights of a call in q's type or in fp32)
             if w.data_ptr() % 16:
                 w = w.clone()
-                keep.append(w)
+            keep.append(w)
             a.weight[i], a.w_dtype[i] = w.data_ptr(), _IN_DTYPE[w.dtype]
         outs.append(y)
         keep.append(x)

@@ -45,7 +45,8 @@ def _set(a, name, value):
 
 
 @pytest.mark.parametrize("change", [dict(x=(0, None)), dict(y=(0, None)), dict(x=(1, ADDRESS)), dict(x=(0, ADDRESS + 2)), dict(in_dtype=3), dict(D=96), dict(B=0),
-                                    dict(L=-1), dict(H=(0, 0)), dict(norm=3), dict(eps=-1.0), dict(eps=float("nan")), dict(x_sl=(0, 130)), dict(w_dtype=(0, 5)),
+                                    dict(L=-1), dict(H=(0, 0)), dict(norm=3), dict(eps=-1.0), dict(eps=float("nan")), dict(x_sl=(0, 130)), dict(weight=(0, ADDRESS), w_dtype=(0, 5)),
+                                    dict(weight=(0, ADDRESS), w_dtype=(0, 1)), dict(weight=(0, ADDRESS + 8)),
                                     dict(sin=None), dict(rot=0), dict(rot=12), dict(rot=136), dict(table_rows=0), dict(cos=ADDRESS + 4), dict(axes=0),
                                     dict(axes=2), dict(axes=5), dict(B=70000, L=70000)], ids=str)
 def test_norm_rope_refuses(change):
