@@ -355,6 +355,7 @@ int mpsa_kv_read(const mpsa_kv_read_args* args, void* stream);
  *   mask      bytes [B or 1, T, T], batch stride mask_sb, dense rows
  *   lse       optional fp32 [B,Hq,T] dense: log2 of each row's softmax denominator, as in mpsa_attn_fwd
  *   workspace mpsa_kv_attention_workspace bytes, 256-byte aligned, private to the call until it has finished on the GPU
+ *   status    as in mpsa_attn_fwd
  * Rows that see no key, and rows from q_lens[b] on, give zero (lse -inf). */
 typedef struct mpsa_kv_attention_args {
   mpsa_kv_cache cache;
@@ -366,6 +367,7 @@ typedef struct mpsa_kv_attention_args {
   long long q_sb, q_sh, q_sl, o_sb, o_sh, o_sl, table_sb, mask_sb;
   const int *page_table, *lengths, *q_lens;
   const unsigned char* mask;
+  int* status;
   int dtype, B, T, Hq, max_pages;
   float sm_scale;
 } mpsa_kv_attention_args;

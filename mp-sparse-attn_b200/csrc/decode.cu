@@ -1,11 +1,7 @@
 // Attention of a sequence's last tokens over its paged MX cache (mpsa_kv_attention).
 //
-// A unit of work is one sequence, one KV head and up to 8 NR of its query rows (row r = token r / G, query head r % G of the KV head's G).
-// A step is 32 keys.  The steps of all units, laid end to end, are cut into equal runs, one per CTA, whatever the lengths are: CTAs compute
-// the cut from the lengths in device memory.  A unit that falls to several CTAs leaves parts (fp32 sums with their row references and
-// denominators), which the combining kernel adds up in the order of the keys.
-//
-// Within a CTA the warps take steps in turn and have nothing to do with each other until the run's part of a unit is done: each copies its own
+// This kernel: up to 32 query rows of a KV head, steps of 32 keys (decode.cuh says what a unit, a step and a run are; decode_wide.cu has the
+// kernel for more rows).  Within a CTA the warps take steps in turn and have nothing to do with each other until the run's part of a unit is done: each copies its own
 // keys to its own shared memory with cp.async, and keeps its own references, sums and output in registers.
 //
 //   scores    S^T = K Q^T by m16n8k16 on fp16 operands, keys in the M dimension: a few query rows fill the N of 8.  Element codes convert
@@ -22,62 +18,17 @@
 //
 // It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each.
 #include "api_internal.h"
-#include "common.cuh"
-#include "serving.cuh"
+#include "decode.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mpsa {
 namespace {
 
 constexpr int kWarps = 4, kStep = 32;
-constexpr int kMinShare = 4;                   // steps of a run at least: one for each warp
 constexpr float kMost = 15.0f, kSet = 7.0f;    // log2 of the largest product that raises no reference, and of the largest one after a raise
 constexpr int kLeast = -85;                    // log2 of a scale that counts as that at least: references are the largest score - 100 at least
-
-struct Call : mpsa_kv_attention_args {
-  int tiles;                                   // NR: row tiles of 8 in a unit
-  int groups;                                  // units of a (sequence, KV head)
-  float* part;                                 // [2 x CTAs][8 NR][D], a CTA's run has at most two units that it shares with others
-  float2* stat;                                // [2 x CTAs][8 NR]: row reference (log2), denominator relative to it
-};
-
-__device__ __forceinline__ int length_of(const Call& a, int b) {
-  return min(max(a.lengths[b], 0), (int)min(0x7fffffc0ll, (long long)a.max_pages * a.cache.page_size));
-}
-__device__ __forceinline__ int queries_of(const Call& a, int b, int len) { return min(a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T, len); }
-__device__ __forceinline__ int steps_of(int len) { return max(1, (len + kStep - 1) / kStep); }    // (an empty sequence: one, which writes its zeros)
-
-// How many steps of all units a CTA takes (`share`), the sequence that step cta * share belongs to (returned; a.B: beyond the last) and where
-// that sequence's steps begin.  By a whole warp; plan() has seen to it that the steps of all units fit 32 bits.
-__device__ int locate(const Call& a, uint32_t ctas, uint32_t cta, uint32_t& share, uint32_t& begin, int lane) {
-  const uint32_t units = a.cache.Hkv * a.groups;
-  const uint32_t mine = lane < a.B ? steps_of(length_of(a, lane)) * units : 0;       // the first 32 sequences: read once
-  uint32_t sum = mine;
-  for (int b = lane + 32; b < a.B; b += 32) sum += steps_of(length_of(a, b)) * units;
-  sum = __reduce_add_sync(0xffffffffu, sum);
-  share = max((sum + ctas - 1) / ctas, (uint32_t)kMinShare);
-  const unsigned long long want = (unsigned long long)cta * share;
-  begin = 0;
-  if (want >= sum) return a.B;
-  const uint32_t at = (uint32_t)want;
-  for (int b0 = 0;; b0 += 32) {
-    const uint32_t n = b0 == 0 ? mine : b0 + lane < a.B ? steps_of(length_of(a, b0 + lane)) * units : 0;
-    uint32_t up = n;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, up, d);
-      if (lane >= d) up += v;
-    }
-    const unsigned beyond = __ballot_sync(0xffffffffu, begin + up > at);
-    if (beyond) {
-      const int l = __ffs(beyond) - 1;
-      begin += __shfl_sync(0xffffffffu, up - n, l);
-      return b0 + l;
-    }
-    begin += __shfl_sync(0xffffffffu, up, 31);
-  }
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -87,12 +38,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {       // zeros where it is not
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
 }
@@ -187,7 +132,7 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
   uint32_t at = blockIdx.x * share;
   const uint32_t stop = at + min(share, ~at);
   for (bool again = false; b < a.B && at < stop; again = true) {
-    const int len = length_of(a, b), steps = steps_of(len);
+    const int len = length_of(a, b), steps = steps_of(a, len);
     const uint32_t off = at - begin;
     const int u = off / (uint32_t)steps, s0 = off - u * (uint32_t)steps, s1 = min((uint32_t)steps, s0 + (stop - at));
     const int h = u / a.groups, row0 = u % a.groups * Y::rows;
@@ -551,13 +496,13 @@ template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_constant__ Call a, int ctas) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, units = a.cache.Hkv * a.groups;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
-  const int rows = 8 * a.tiles, r = blockIdx.y * kWarps + warp, G = a.Hq / a.cache.Hkv, row = u % a.groups * rows + r;
+  const int rows = a.rows, r = blockIdx.y * kWarps + warp, G = a.Hq / a.cache.Hkv, row = u % a.groups * rows + r;
   uint32_t share, begin;
   locate(a, ctas, 0, share, begin, lane);
   begin = 0;
-  for (int i = lane; i < b; i += 32) begin += steps_of(length_of(a, i)) * units;
+  for (int i = lane; i < b; i += 32) begin += steps_of(a, length_of(a, i)) * units;
   begin = __reduce_add_sync(0xffffffffu, begin);
-  const int len = length_of(a, b), steps = steps_of(len), ql = queries_of(a, b, len);
+  const int len = length_of(a, b), steps = steps_of(a, len), ql = queries_of(a, b, len);
   begin += u * steps;
   const int c0 = begin / share, parts = (begin + steps - 1) / share - c0 + 1;
   grid_dependency_wait();                             // (by everybody: what follows on the stream counts on it)
@@ -607,35 +552,41 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
   if (a.lse && lane == 0) static_cast<float*>(a.lse)[((long long)b * a.Hq + hq) * a.T + tok] = none ? -INFINITY : top + log2f(sum);
 }
 
+bool wide(const Call& a) { return a.rows == kWideRows; }
+
 int ctas_of(const Call& a) {                          // of an SM: as many as registers and shared memory let in
-  const long long most = (long long)a.B * a.cache.Hkv * a.groups * (((long long)a.max_pages * a.cache.page_size + kStep - 1) / kStep + 1);
-  const long long all = (a.tiles == 4 ? 2ll : a.tiles == 2 || a.cache.elem != E2M1 ? 3ll : 4ll) * sm_count();
+  const double most = (double)a.B * a.cache.Hkv * a.groups * ((double)a.max_pages * a.cache.page_size / a.step + 1);
+  const double all = (double)(wide(a) ? kWideCtas : a.rows == 32 ? 2 : a.rows == 16 || a.cache.elem != E2M1 ? 3 : 4) * sm_count();
   return (int)(most < all ? most : all);
 }
 
 template <typename T, int ELEM, int D, int NR>
-int launch(const Call& a, cudaStream_t st) {
+int launch(const Call& a, int ctas, cudaStream_t st) {
   constexpr int bytes = Layout<ELEM, D, NR>::bytes;
   constexpr int id = (std::is_same_v<T, __half> ? 10000 : 0) + ELEM * 1000 + D * 8 + NR;
-  const int ctas = ctas_of(a);
   if (!allow_smem<id>(kv_attention_kernel<T, ELEM, D, NR>, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
   kv_attention_kernel<T, ELEM, D, NR><<<ctas, 32 * kWarps, bytes, st>>>(a);
-  if (int rc = check_launch("kv_attention")) return rc;
-  const dim3 grid(a.B * a.cache.Hkv * a.groups, 2 * NR);
-  launch_dependent(kv_combine_kernel<T, D>, grid, 32 * kWarps, 0, st, true, a, ctas);
   return check_launch("kv_attention");
 }
 template <typename T, int ELEM, int D>
-int launch_tiles(const Call& a, cudaStream_t st) {
-  return a.tiles == 1 ? launch<T, ELEM, D, 1>(a, st) : a.tiles == 2 ? launch<T, ELEM, D, 2>(a, st) : launch<T, ELEM, D, 4>(a, st);
+int launch_rows(const Call& a, int ctas, cudaStream_t st) {
+  return a.rows == 8 ? launch<T, ELEM, D, 1>(a, ctas, st) : a.rows == 16 ? launch<T, ELEM, D, 2>(a, ctas, st) : launch<T, ELEM, D, 4>(a, ctas, st);
 }
 template <typename T, int ELEM>
-int launch_depth(const Call& a, cudaStream_t st) {
-  return a.cache.D == 64 ? launch_tiles<T, ELEM, 64>(a, st) : launch_tiles<T, ELEM, 128>(a, st);
+int launch_depth(const Call& a, int ctas, cudaStream_t st) {
+  return a.cache.D == 64 ? launch_rows<T, ELEM, 64>(a, ctas, st) : launch_rows<T, ELEM, 128>(a, ctas, st);
 }
 template <typename T>
-int launch_elem(const Call& a, cudaStream_t st) {
-  return a.cache.elem == E4M3 ? launch_depth<T, E4M3>(a, st) : a.cache.elem == E5M2 ? launch_depth<T, E5M2>(a, st) : launch_depth<T, E2M1>(a, st);
+int launch_all(const Call& a, cudaStream_t st) {
+  const int ctas = ctas_of(a), elem = a.cache.elem;
+  if (int rc = wide(a) ? launch_wide(a, ctas, st)
+                       : elem == E4M3 ? launch_depth<T, E4M3>(a, ctas, st) : elem == E5M2 ? launch_depth<T, E5M2>(a, ctas, st) : launch_depth<T, E2M1>(a, ctas, st))
+    return rc;
+  const int rows = a.T * (a.Hq / a.cache.Hkv);
+  const dim3 grid(a.B * a.cache.Hkv * a.groups, (std::min(rows, a.rows) + kWarps - 1) / kWarps);
+  if (a.cache.D == 64) launch_dependent(kv_combine_kernel<T, 64>, grid, 32 * kWarps, 0, st, true, a, ctas);
+  else launch_dependent(kv_combine_kernel<T, 128>, grid, 32 * kWarps, 0, st, true, a, ctas);
+  return check_launch("kv_attention");
 }
 
 // The call with its plan and its workspace's parts; the workspace's bytes, or an error.
@@ -650,11 +601,13 @@ long long plan(const mpsa_kv_attention_args* args, Call& a) {
   if (a.B > 65535 || a.Hq > 65535 || a.T > 1024) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: at most 65535 sequences and 1024 query tokens");
   if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: sm_scale must be positive and finite");
   const int rows = a.T * (a.Hq / a.cache.Hkv);
-  a.tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  a.groups = (rows + 8 * a.tiles - 1) / (8 * a.tiles);
-  const double most = (double)a.B * a.cache.Hkv * a.groups * (((double)a.max_pages * a.cache.page_size) / kStep + 1);
-  if (most > 4e9) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: sequences x heads x page table too large (%.1e steps of %d keys, at most 4e9)", most, kStep);
-  const long long slots = 2ll * ctas_of(a) * 8 * a.tiles;
+  a.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : kWideRows;
+  a.step = wide(a) ? kWideStep : kStep;
+  a.least = wide(a) ? 2 : 4;                          // (four: a step for each warp)
+  a.groups = (rows + a.rows - 1) / a.rows;
+  const double most = (double)a.B * a.cache.Hkv * a.groups * ((double)a.max_pages * a.cache.page_size / a.step + 1);
+  if (most > 4e9) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: sequences x heads x page table too large (%.1e steps of %d keys, at most 4e9)", most, a.step);
+  const long long slots = 2ll * ctas_of(a) * a.rows;
   a.part = static_cast<float*>(a.workspace);
   a.stat = reinterpret_cast<float2*>(a.part + slots * a.cache.D);
   return slots * (a.cache.D * 4 + 8);
@@ -674,11 +627,11 @@ extern "C" int mpsa_kv_attention(const mpsa_kv_attention_args* args, void* strea
   Call a;
   const long long need = plan(args, a);
   if (need < 0) return (int)need;
-  if (!a.q || !a.out) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: null pointer");
+  if (!a.q || !a.out || !a.status) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: null pointer");
   if ((a.q_sb | a.q_sh | a.q_sl | a.o_sb | a.o_sh | a.o_sl) % 8 || ((uintptr_t)a.q | (uintptr_t)a.out) % 16)
     return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: q and out need 16-byte aligned bases and strides that are multiples of 8 elements");
   if (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 256)
     return set_error(MPSA_ERR_BAD_ARG, "kv_attention: the workspace must hold %lld bytes and be 256-byte aligned", need);
   const cudaStream_t st = (cudaStream_t)stream;
-  return a.dtype == 0 ? launch_elem<__nv_bfloat16>(a, st) : launch_elem<__half>(a, st);
+  return a.dtype == 0 ? launch_all<__nv_bfloat16>(a, st) : launch_all<__half>(a, st);
 }

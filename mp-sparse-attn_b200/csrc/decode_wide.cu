@@ -1,0 +1,506 @@
+// Attention of many query rows over a paged MX cache (mpsa_kv_attention with more than 32 rows of a KV head: trees of drafted tokens, short
+// chunks) on the 5th-generation tensor cores.
+//
+// A unit is up to 128 query rows, a step 128 keys.  Nine warps: 4 convert, 4 are the softmax, one issues the tensor operations.
+//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory.  K relative
+//             to the largest scale of its 32 keys (a factor of the scores), V relative to the largest of its key (a factor of P): what fp16
+//             cannot hold is 2^-30 of that.  Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an
+//             MN-major one.
+//   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
+//   softmax   a thread a row: the row's reference U, set and raised as decode.cu says; P times V's factor, rounded to fp16, goes over S.
+//   P V       128 x D x 128, P from TMEM, added up in TMEM.
+// One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
+// It is bound by the softmax warps' issue and the exponentials (16 a clock and SM, 1024 cycles a step).
+#include "api_internal.h"
+#include "decode.cuh"
+
+#include <type_traits>
+
+namespace mpsa {
+namespace {
+
+constexpr int kThreads = 288, kColumns = 256;          // TMEM: S, over it P, then O from column 128
+constexpr float kMost = 15.0f, kSet = 7.0f;            // as in decode.cu
+constexpr int kLeast = -85;
+
+template <int D>
+struct Layout {
+  static constexpr int half = 128 * 128;               // 64 depth elements of 128 rows
+  static constexpr int tile = half * (D / 64);
+  static constexpr int q = 0, k = tile, v = 2 * tile, vectors = 3 * tile;
+  // two steps' worth of: factors of P and log2 of them for 128 keys
+  static constexpr int bytes = vectors + 2 * 2 * 128 * 4 + 1024;       // (and what aligning the base may take)
+};
+
+struct Shared {
+  uint64_t k_full, v_full, s_full, p_full, pv_done, q_full, drained;
+  uint32_t tmem;
+  float k_size[2][4];                                  // 2^(largest scale of 32 keys)
+  uint32_t there[2][4];                                // keys with a page and within the length
+  uint32_t strange[2][4][4];                           // [32 keys][block of the depth]: scales of V that are NaN
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+               "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void store_shared16(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// 2^d in both halves (0 below 2^-24), d at most 0
+__device__ __forceinline__ uint32_t power2(int d) { return pack2(__half(), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23)); }
+
+// The parts of a unit that a CTA's run covers, one after the other, for each role alike.
+struct Run {
+  uint32_t at, stop, begin;
+  int b;
+  int len, steps, u, s0, s1, h, row0, ql, first;
+  __device__ __forceinline__ Run(const Call& a, int lane) {
+    uint32_t share;
+    b = locate(a, gridDim.x, blockIdx.x, share, begin, lane);
+    at = blockIdx.x * share;
+    stop = at + min(share, ~at);
+  }
+  __device__ __forceinline__ bool next(const Call& a) {
+    if (b >= a.B || at >= stop) return false;
+    len = length_of(a, b);
+    steps = steps_of(a, len);
+    const uint32_t off = at - begin, units = a.cache.Hkv * a.groups;
+    u = off / (uint32_t)steps;
+    s0 = off - u * (uint32_t)steps;
+    s1 = min((uint32_t)steps, s0 + (stop - at));
+    h = u / a.groups;
+    row0 = u % a.groups * kWideRows;
+    ql = queries_of(a, b, len);
+    first = len - ql;
+    at += s1 - s0;
+    now = b;
+    if (at - begin >= (uint32_t)steps * units) {
+      begin += (uint32_t)steps * units;
+      ++b;
+    }
+    return true;
+  }
+  int now;                                             // the sequence
+};
+
+// Keys on their way: a warp's 32 rows of K or V, and the scale codes of key `lane`
+template <int ELEM, int D>
+struct Rows {
+  static constexpr int row = code_bytes(ELEM, D), cpr = row / 16, rpi = 32 / cpr;       // 16-byte pieces of a row, rows of one load
+  uint4 code[cpr];
+  uint32_t scale;
+};
+
+// pos: the warp's first key; a lane's page is that of key pos + lane
+template <int ELEM, int D>
+__device__ __forceinline__ void request(Rows<ELEM, D>& r, const mpsa_kv_cache& c, const void* codes, const void* scales, int h, int pos, int page, bool there, int lane) {
+  using R = Rows<ELEM, D>;
+  const long long at = ((long long)max(page, 0) * c.Hkv + h) * c.page_size + ((pos + lane) & (c.page_size - 1));
+  r.scale = 0;
+  if (there) r.scale = D == 128 ? static_cast<const uint32_t*>(scales)[at] : static_cast<const unsigned short*>(scales)[at];
+#pragma unroll
+  for (int i = 0; i < R::cpr; ++i) {
+    const int key = i * R::rpi + lane / R::cpr;
+    const long long from = __shfl_sync(0xffffffffu, there ? at : -1ll, key);
+    r.code[i] = make_uint4(0, 0, 0, 0);
+    if (from >= 0) r.code[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(codes) + from * R::row + lane % R::cpr * 16);
+  }
+}
+
+// fp16 rows into shared memory; `ref` (of lane's key) is subtracted from the scale codes; nan: what a NaN scale becomes
+template <int ELEM, int D>
+__device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, int ref, uint32_t nan, int lane) {
+  using R = Rows<ELEM, D>;
+  const int ch = lane % R::cpr, blk = ELEM == E2M1 ? ch : ch / 2;
+#pragma unroll
+  for (int i = 0; i < R::cpr; ++i) {
+    const int key = i * R::rpi + lane / R::cpr, row = row0 + key;
+    const uint32_t e = __shfl_sync(0xffffffffu, r.scale, key) >> (8 * blk) & 255u;
+    const int base = __shfl_sync(0xffffffffu, ref, key);
+    const uint32_t f = e == 255u ? nan : power2((int)e - base);
+    const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
+    if constexpr (ELEM == E2M1) {                      // 32 elements, 64 bytes
+      const uint32_t to = tile + ch / 2 * (128 * 128) + row * 128;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x[4];
+        elem_quads(w[j], x[0], x[1], x[2], x[3]);
+        store_shared16(to + ((ch % 2 * 4 + j) ^ (row & 7)) * 16, times(x[0], f), times(x[1], f), times(x[2], f), times(x[3], f));
+      }
+    } else {                                           // 16 elements, 32 bytes; lanes of the upper half of the depth write their second piece first
+      const uint32_t to = tile + ch / 4 * (128 * 128) + row * 128;
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        elem_two<ELEM>(w[j], x[2 * j], x[2 * j + 1]);
+        x[2 * j] = times(x[2 * j], f);
+        x[2 * j + 1] = times(x[2 * j + 1], f);
+      }
+      const bool late = D == 128 && ch >= 4;
+      const int c0 = ch % 4 * 2 + late, c1 = ch % 4 * 2 + !late;
+      store_shared16(to + (c0 ^ (row & 7)) * 16, late ? x[4] : x[0], late ? x[5] : x[1], late ? x[6] : x[2], late ? x[7] : x[3]);
+      store_shared16(to + (c1 ^ (row & 7)) * 16, late ? x[0] : x[4], late ? x[1] : x[5], late ? x[2] : x[6], late ? x[3] : x[7]);
+    }
+  }
+}
+
+template <typename T, int ELEM, int D>
+__global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(const __grid_constant__ Call a) {
+  using Y = Layout<D>;
+  constexpr int NB = D / 32;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  uint8_t* const smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
+  float* const vectors = reinterpret_cast<float*>(smem + Y::vectors);  // [parity][0: factor, 1: log2][key]
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int G = a.Hq / a.cache.Hkv, R = a.T * G;
+
+  grid_dependents_go();
+  if (warp == 8) {
+    tmem_alloc(&sh.tmem, kColumns);
+    if (lane == 0) {
+      mbar_init(&sh.k_full, 128);
+      mbar_init(&sh.v_full, 128);
+      mbar_init(&sh.s_full, 1);
+      mbar_init(&sh.p_full, 128);
+      mbar_init(&sh.pv_done, 1);
+      mbar_init(&sh.q_full, 128);
+      mbar_init(&sh.drained, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  Run run(a, lane);
+  uint32_t n = 0;                                      // steps so far: every barrier but q_full completes once a step
+  uint32_t units = 0;
+  bool ok = true;
+
+  if (warp < 4) {
+    // ---- softmax: row warp * 32 + lane of the unit
+    const uint32_t mine = tmem + (uint32_t)(warp * 32) * 65536u;
+    for (; ok && run.next(a); ++units) {
+      const int r = run.row0 + warp * 32 + lane, tok = r / G, hq = run.h * G + r % G;
+      const bool live = r < R, busy = run.row0 + warp * 32 < R;        // busy: the warp has rows
+      // queries (every Q K^T of the unit before is over: this thread has seen its scores)
+      float rs = 0.0f;
+      {
+        const T* q = static_cast<const T*>(a.q) + (run.now * a.q_sb + hq * a.q_sh + (long long)tok * a.q_sl);
+        uint32_t amax = 0;
+        if (live)
+          for (int i = 0; i < D / 4; ++i) {
+            float x[4];
+            load4(q + 4 * i, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+          }
+        const int e = min(max((int)(amax >> 23), 1), 253);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+        rs = amax >= 0x7f800000u ? __int_as_float(0x7fffffff) : a.sm_scale * 1.44269504f * __uint_as_float((uint32_t)e << 23);
+        const int row = warp * 32 + lane;
+        const uint32_t to = smem_u32(smem + Y::q) + row * 128;
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          float x[4] = {}, y[4] = {};
+          if (live) {
+            load4(q + 8 * i, x);
+            load4(q + 8 * i + 4, y);
+          }
+          store_shared16(to + i / 8 * Y::half + ((i % 8) ^ (row & 7)) * 16, pack2(__half(), x[0] * down, x[1] * down), pack2(__half(), x[2] * down, x[3] * down),
+                         pack2(__half(), y[0] * down, y[1] * down), pack2(__half(), y[2] * down, y[3] * down));
+        }
+        fence_proxy_async_smem();
+        const uint32_t zero[16] = {};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) tmem_st16(mine + 128 + 16 * i, zero);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sh.q_full);
+      }
+      float U = -INFINITY, l = 0.0f;
+      for (int s = run.s0; s < run.s1; ++s, ++n) {
+        if (!(ok = mbar_wait(&sh.s_full, n & 1, a.status, KS_TIMEOUT_MMA))) break;
+        tc_fence_after();
+        const int par = n & 1, pos = s * kWideStep;
+        const float *vf = vectors + par * 256, *vl = vf + 128;
+        if (busy) {
+          const bool special = pos + kWideStep > (a.T > 1 || a.mask ? run.first : run.len) ||
+                               (sh.there[par][0] & sh.there[par][1] & sh.there[par][2] & sh.there[par][3]) != 0xffffffffu;
+          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};      // keys that this row sees
+          if (special) {
+            const unsigned char* const mk = a.mask + run.now * a.mask_sb + (long long)tok * a.T;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v = 0;
+              for (int i = 0; i < 32; ++i) {
+                const int j = pos + 32 * c + i - run.first;
+                const bool seen = j < 0 || (live && tok < run.ql && j < run.ql && (a.mask ? mk[j] != 0 : j <= tok));
+                v |= (uint32_t)seen << i;
+              }
+              vis[c] = v & sh.there[par][c];
+            }
+          }
+          float f[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) f[c] = rs * sh.k_size[par][c];
+          // the largest product
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld32(mine + 32 * c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 z = *reinterpret_cast<const float4*>(vl + 32 * c + i);
+              float y[4] = {fmaf(__uint_as_float(x[i]), f[c], z.x), fmaf(__uint_as_float(x[i + 1]), f[c], z.y), fmaf(__uint_as_float(x[i + 2]), f[c], z.z),
+                            fmaf(__uint_as_float(x[i + 3]), f[c], z.w)};
+              if (special)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (!(vis[c] >> (i + e) & 1)) y[e] = -INFINITY;
+              top = fmaxf(top, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+            }
+          }
+          const bool raise = top > U + kMost;
+          if (__any_sync(0xffffffffu, raise)) {
+            const float up = raise ? top - kSet : U, w = raise ? exp2_fast(U - up) : 1.0f;
+            if (__any_sync(0xffffffffu, raise && U != -INFINITY)) {   // (P V of the step before is over: Q K^T was issued behind it)
+#pragma unroll 1
+              for (int i = 0; i < D / 16; ++i) {
+                uint32_t x[16];
+                tmem_ld16(mine + 128 + 16 * i, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * w);
+                tmem_st16(mine + 128 + 16 * i, x);
+              }
+            }
+            l *= w;
+            U = up;
+          }
+          const float ref = U == -INFINITY ? 0.0f : U;
+          // P times V's factors over S: columns 16c .. of the 32c .. that have been read
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32], p[16];
+            tmem_ld32(mine + 32 * c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 z = *reinterpret_cast<const float4*>(vf + 32 * c + i);
+              float y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f[c], -ref));
+                if (special && !(vis[c] >> (i + e) & 1)) y[e] = 0.0f;
+              }
+              l += (y[0] + y[1]) + (y[2] + y[3]);
+              p[i / 2] = pack2(__half(), y[0] * z.x, y[1] * z.y);
+              p[i / 2 + 1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
+            }
+            tmem_st16(mine + 16 * c, p);
+          }
+          // a value that is NaN: its block of the depth is, in the rows that see it
+          uint32_t any = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) any |= sh.strange[par][c][i];
+          if (any) {
+            tmem_st_wait();
+#pragma unroll 1
+            for (int i = 0; i < NB; ++i) {
+              uint32_t hit = 0;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) hit |= sh.strange[par][c][i] & vis[c];
+#pragma unroll 1
+              for (int y = 0; y < 2; ++y) {
+                uint32_t x[16];
+                tmem_ld16(mine + 128 + 32 * i + 16 * y, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = hit ? 0x7fffffffu : x[e];
+                tmem_st16(mine + 128 + 32 * i + 16 * y, x);
+              }
+            }
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(&sh.p_full);
+      }
+      if (!ok || !(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;
+      tc_fence_after();
+      if (!busy) continue;
+      const bool whole = run.s0 == 0 && run.s1 == run.steps;
+      const long long slot = (2ll * blockIdx.x + (run.s0 == 0)) * kWideRows + warp * 32 + lane;
+      const bool none = l == 0.0f || tok >= run.ql;
+      const float w = !whole ? 1.0f : none ? 0.0f : 1.0f / l;
+      T* const y = static_cast<T*>(a.out) + (run.now * a.o_sb + hq * a.o_sh + (long long)tok * a.o_sl);
+#pragma unroll 1
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t x[16];
+        tmem_ld16(mine + 128 + 16 * i, x);
+        tmem_ld_wait();
+        if (live)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            float z[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) z[d] = whole && none ? 0.0f : __uint_as_float(x[e + d]) * w;
+            if (whole) store4(y + 16 * i + e, z);
+            else store4(a.part + slot * D + 16 * i + e, z);
+          }
+      }
+      tc_fence_before();
+      if (live) {
+        if (!whole) a.stat[slot] = make_float2(U, l);
+        else if (a.lse) static_cast<float*>(a.lse)[((long long)run.now * a.Hq + hq) * a.T + tok] = none ? -INFINITY : U + log2f(l);
+      }
+    }
+  } else if (warp < 8) {
+    // ---- conversion: keys 32 (warp - 4) .. of every step
+    const int w = warp - 4;
+    const mpsa_kv_cache& c = a.cache;
+    Rows<ELEM, D> k, v;
+    Run ahead = run;                                   // one step ahead of `run`: what is requested
+    bool more = ahead.next(a);
+    int as = more ? ahead.s0 : 0, page = -1, pos = 0;
+    bool there = false;
+    auto look_up = [&]() {                             // the next step's keys
+      pos = kWideStep * as + 32 * w;
+      page = more ? page_of(a.page_table + ahead.now * a.table_sb, (pos + lane) / c.page_size, a.max_pages, c.num_pages) : -1;
+      there = page >= 0 && pos + lane < ahead.len;
+    };
+    look_up();
+    request<ELEM, D>(k, c, c.k, c.k_scale, ahead.h, pos, page, there, lane);
+    request<ELEM, D>(v, c, c.v, c.v_scale, ahead.h, pos, page, there, lane);
+    while (ok && run.next(a))
+      for (int s = run.s0; s < run.s1; ++s, ++n) {
+        const int par = n & 1;
+        const bool here = there;
+        if (more && ++as == ahead.s1) {                // what comes after this step
+          more = ahead.next(a);
+          as = more ? ahead.s0 : 0;
+        }
+        look_up();
+        if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
+        // K: one reference for the warp's keys
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const uint32_t e = k.scale >> (8 * i) & 255u;
+          top = max(top, e == 255u ? 0u : e);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        convert<ELEM, D>(k, smem_u32(smem + Y::k), 32 * w, (int)top, 0x7fff7fffu, lane);
+        // V: one for each key
+        uint32_t vtop = 0;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const uint32_t e = v.scale >> (8 * i) & 255u;
+          vtop = max(vtop, e == 255u ? 0u : e);
+          const uint32_t strange = __ballot_sync(0xffffffffu, e == 255u);
+          if (lane == 0) sh.strange[par][w][i] = strange;
+        }
+        vectors[par * 256 + 32 * w + lane] = scale_value(vtop);
+        vectors[par * 256 + 128 + 32 * w + lane] = (float)max((int)vtop - 127, kLeast);
+        const uint32_t has = __ballot_sync(0xffffffffu, here);
+        if (lane == 0) {
+          sh.there[par][w] = has;
+          sh.k_size[par][w] = scale_value(top);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.k_full);
+        request<ELEM, D>(k, c, c.k, c.k_scale, ahead.h, pos, page, there, lane);
+        if (n > 0 && !(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;     // V is free
+        convert<ELEM, D>(v, smem_u32(smem + Y::v), 32 * w, (int)vtop, 0u, lane);
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.v_full);
+        request<ELEM, D>(v, c, c.v, c.v_scale, ahead.h, pos, page, there, lane);
+      }
+  } else {
+    // ---- tensor operations
+    constexpr uint32_t kQk = idesc_f16(0, 0, 128, 128), kPv = idesc_f16(0, 0, 128, D) | 1u << 16;     // (bit 16: B is MN-major)
+    const uint32_t q = smem_u32(smem + Y::q), k = smem_u32(smem + Y::k), v = smem_u32(smem + Y::v);
+    for (; ok && run.next(a); ++units) {
+      ok = mbar_wait(&sh.q_full, units & 1, a.status, KS_TIMEOUT_PIPE);
+      for (int s = run.s0; ok && s < run.s1; ++s, ++n) {
+        // S is free when P V of the step before has read P
+        ok = mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE) && (n == 0 || mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            mma_f16_ss(tmem, sdesc_kmajor_sw128(q + i / 4 * Y::half + i % 4 * 32), sdesc_kmajor_sw128(k + i / 4 * Y::half + i % 4 * 32), kQk, i > 0);
+          tc_commit(&sh.s_full);
+        }
+        __syncwarp();
+        ok = mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) && mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mma_f16_ts(tmem + 128, tmem + 8 * i, make_sdesc(v + i * 2048, Y::half, 1024, kLayoutSw128), kPv, 1);
+          tc_commit(&sh.pv_done);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {                                         // what has been issued ends before its memory goes
+      if (elect_one()) {
+        tc_commit(&sh.drained);
+        mbar_drain(&sh.drained, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, kColumns);
+}
+
+template <typename T, int ELEM, int D>
+int launch(const Call& a, int ctas, cudaStream_t st) {
+  constexpr int id = 100000 + (std::is_same_v<T, __half> ? 1 : 0) + ELEM * 10 + D * 100;
+  if (!allow_smem<id>(kv_attention_wide_kernel<T, ELEM, D>, Layout<D>::bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
+  kv_attention_wide_kernel<T, ELEM, D><<<ctas, kThreads, Layout<D>::bytes, st>>>(a);
+  return check_launch("kv_attention");
+}
+template <typename T, int ELEM>
+int launch_depth(const Call& a, int ctas, cudaStream_t st) {
+  return a.cache.D == 64 ? launch<T, ELEM, 64>(a, ctas, st) : launch<T, ELEM, 128>(a, ctas, st);
+}
+template <typename T>
+int launch_elem(const Call& a, int ctas, cudaStream_t st) {
+  return a.cache.elem == E4M3 ? launch_depth<T, E4M3>(a, ctas, st) : a.cache.elem == E5M2 ? launch_depth<T, E5M2>(a, ctas, st) : launch_depth<T, E2M1>(a, ctas, st);
+}
+
+}  // namespace
+
+int launch_wide(const Call& a, int ctas, cudaStream_t st) { return a.dtype == 0 ? launch_elem<__nv_bfloat16>(a, ctas, st) : launch_elem<__half>(a, ctas, st); }
+
+}  // namespace mpsa

@@ -462,16 +462,17 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// kv_attention(cache, cache_k, q, page_table, lengths, q_lens, mask, sm_scale, want_lse, hnd) -> out or (out, lse)
+// kv_attention(cache, cache_k, q, page_table, lengths, q_lens, mask, status, sm_scale, want_lse, hnd) -> out or (out, lse)
 PyObject* kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!counted(n, 10, "kv_attention")) return nullptr;
+  if (!counted(n, 11, "kv_attention")) return nullptr;
   return guarded([&]() -> PyObject* {
     const mpsa_kv_cache* cache = cache_of(a[0]);
     const at::Tensor *own = plain(a[1]), *q = plain(a[2]), *table = plain(a[3]), *lengths = plain(a[4]), *qlens, *mask;
     if (!cache || !own || !q || !table || !lengths || !optional_plain(a[5], qlens) || !optional_plain(a[6], mask)) Py_RETURN_NONE;
     mpsa_kv_attention_args c = {};
-    c.sm_scale = (float)PyFloat_AsDouble(a[7]);
-    const int lse = PyObject_IsTrue(a[8]), hnd = PyObject_IsTrue(a[9]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
+    c.status = static_cast<int*>(PyLong_AsVoidPtr(a[7]));
+    c.sm_scale = (float)PyFloat_AsDouble(a[8]);
+    const int lse = PyObject_IsTrue(a[9]), hnd = PyObject_IsTrue(a[10]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
     if (PyErr_Occurred()) return nullptr;
     c.dtype = in_dtype(*q);
     if (c.dtype < 0 || !rows_aligned(*q, 8) || q->get_device() != device || q->size(3) != cache->D || q->size(h) % cache->Hkv || q->size(l) > 1024) Py_RETURN_NONE;

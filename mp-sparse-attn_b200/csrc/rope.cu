@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 4) norm_rope_heads_kernel(const __gr
 // sum and the rest.  Few threads a token and many CTAs an SM: the others' loads run under one's barrier.
 constexpr int kChunks = 8;
 template <typename T, typename W, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(512) norm_rope_across_kernel(const __grid_constant__ NormRope a) {
+__global__ void __launch_bounds__(256, 3) norm_rope_across_kernel(const __grid_constant__ NormRope a) {
   __shared__ float part[16];
   __shared__ __align__(16) float angle[2][4 * LANES];
   const int o = blockIdx.y, H = a.H[o];

@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _IN_DTYPE, _OUT_DTYPE, _bhld, _on_device, _ptr, _require_cuda
+from .ops import _IN_DTYPE, _OUT_DTYPE, _bhld, _on_device, _ptr, _raise_if_failed, _require_cuda, _state
 
 _ELEM = {"e4m3": 0, "e5m2": 1, "e2m1": 2}
 _c_int, _c_ll, _c_p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
@@ -50,7 +50,7 @@ class _ReadArgs(ctypes.Structure):
 class _AttentionArgs(ctypes.Structure):
     _fields_ = [("cache", _Cache), ("q", _c_p), ("out", _c_p), ("lse", _c_p), ("workspace", _c_p), ("workspace_bytes", _c_ll)] + \
         [(n, _c_ll) for n in ("q_sb", "q_sh", "q_sl", "o_sb", "o_sh", "o_sl", "table_sb", "mask_sb")] + \
-        [(n, _c_p) for n in ("page_table", "lengths", "q_lens", "mask")] + \
+        [(n, _c_p) for n in ("page_table", "lengths", "q_lens", "mask", "status")] + \
         [(n, _c_int) for n in ("dtype", "B", "T", "Hq", "max_pages")] + [("sm_scale", ctypes.c_float)]
 
 
@@ -305,15 +305,18 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     mask: bool [T,T] or [B,T,T], True where query token i sees query token j - a tree of drafted tokens; None: every token sees those before
     it and itself.  Cached tokens before the query tokens are seen by all.  A row that sees nothing is zero.
     return_lse: also fp32 [B,Hq,T], log2 of the softmax denominators (-inf for a row that sees nothing), as attention_merge takes it."""
+    dev = cache.k.device
+    st = _state(dev.index)
+    if st.word.value:
+        _raise_if_failed(dev)
     if tensor_layout in ("HND", "NHD"):
-        r = _lib.native().kv_attention(cache._c, cache.k, q, page_table, lengths, q_lens, mask,
+        r = _lib.native().kv_attention(cache._c, cache.k, q, page_table, lengths, q_lens, mask, st.status_ptr,
                                        cache.head_dim ** -0.5 if sm_scale is None else sm_scale, return_lse, tensor_layout == "HND")
         if r is not None:
             if r.__class__ is int:
                 _lib.check(r)
             return r
     _require_cuda(q, page_table, lengths, q_lens, mask)
-    dev = cache.k.device
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"unsupported query dtype {q.dtype}")
     if q.device != dev:
@@ -335,7 +338,7 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     _, _, os = _bhld(out, tensor_layout)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
     a = _AttentionArgs(cache._block(), q.data_ptr(), out.data_ptr(), _ptr(lse), None, 0, *qs, *os, page_table.stride(0),
-                       0 if mask is None or mask.dim() == 2 else T * T, page_table.data_ptr(), lengths.data_ptr(), _ptr(q_lens), _ptr(mask),
+                       0 if mask is None or mask.dim() == 2 else T * T, page_table.data_ptr(), lengths.data_ptr(), _ptr(q_lens), _ptr(mask), st.status_ptr,
                        _IN_DTYPE[q.dtype], B, T, Hq, page_table.shape[1], sm)
     lib = _lib.load()
     need = lib.mpsa_kv_attention_workspace(ctypes.byref(a))

@@ -52,8 +52,8 @@ def gather(buf, table, length):
 
 
 def attention(q, k, v, seen, sm_scale):
-    """One sequence: q [Hq,T,D], k, v [Hkv,n,D] fp64, seen bool [T,n] -> out [Hq,T,D], log2 denominators [Hq,T], sum p |v| / sum p, and the
-    largest sum |q k| sm_scale of each row."""
+    """One sequence: q [Hq,T,D], k, v [Hkv,n,D] fp64, seen bool [T,n] -> out [Hq,T,D], log2 denominators [Hq,T], sum p |v| / sum p, the
+    largest sum |q k| sm_scale of each row, and the largest p |v| / sum p of each row."""
     G = q.shape[0] // k.shape[0]
     k, v = k.repeat_interleave(G, 0), v.repeat_interleave(G, 0)
     s = (q @ k.transpose(1, 2)) * sm_scale
@@ -65,10 +65,11 @@ def attention(q, k, v, seen, sm_scale):
     # (a key that a row does not see has no part in it, whatever its value is)
     vz = torch.nan_to_num(v)
     o, a = p @ vz, p @ vz.abs()
+    big = (torch.nan_to_num(p) * vz.abs().amax(-1).unsqueeze(1)).amax(-1) if k.shape[1] else torch.zeros(q.shape[:2], dtype=torch.float64)
     for h, t in torch.nonzero(torch.isnan(p).any(-1) | ((p @ torch.isnan(v).any(-1, keepdim=True).double()).squeeze(-1) > 0)).tolist():
         o[h, t] = (p[h, t].unsqueeze(-1) * torch.where(seen[t].unsqueeze(-1), v[h], 0.0)).sum(0)
     o[:, none] = 0.0
-    return o, torch.where(none, float("-inf"), lse / torch.log(torch.tensor(2.0, dtype=torch.float64))), a, mag
+    return o, torch.where(none, float("-inf"), lse / torch.log(torch.tensor(2.0, dtype=torch.float64))), a, mag, big
 
 
 def norm_rope(x, weight, norm, eps, cos, sin, rows, interleaved):

@@ -314,7 +314,10 @@ def check_attention(c, table, lens, q, out, lse, q_lens=None, mask=None, sm=None
 
     A score is a sum of D products in fp32, scaled per block: off by at most (D + 8) 2^-23 of the sum of its terms' magnitudes (a matrix
     instruction may cut off instead of rounding), which moves log2 of a probability by that times log2(e), and the exponential adds 2^-22.
-    P is rounded to fp16 (2^-11), sums of n fp32 terms to n 2^-24 at worst, n up to a few hundred in one accumulator (2^-16); the output is rounded once."""
+    P is rounded to fp16 (2^-11), sums of n fp32 terms to n 2^-24 at worst, n up to a few hundred in one accumulator (2^-16); the output is rounded once.
+    What is rounded is P times a block scale, in units in which the row's largest such product is 2^7 at least: fp16 steps of 2^-24 below 2^-14 add
+    2^-25 for each key, 2^-32 of the largest product.  An element is at most the type's largest value L times its scale, and the largest element of a
+    block more than L/2 times it (the scale is the smallest one that does), so that is 2^-31 of the row's largest p |v|, for each of n keys."""
     B, Hq, T, D = q.shape
     sm = D ** -0.5 if sm is None else sm
     for b in range(B):
@@ -326,12 +329,12 @@ def check_attention(c, table, lens, q, out, lse, q_lens=None, mask=None, sm=None
             seen[:, n - t:] = torch.ones(t, t).tril().bool() if mask is None else (mask if mask.dim() == 2 else mask[b])[:t, :t]
         if absent is not None:
             seen &= ~absent[b][:n]
-        o, l, a, mag = P.attention(q[b, :, :t].double(), k, v, seen, sm)
+        o, l, a, mag, big = P.attention(q[b, :, :t].double(), k, v, seen, sm)
         ds = (D + 8) * 2.0 ** -23 * mag.unsqueeze(-1) + 2.0 ** -22
         got, gl = out[b, :, :t].double(), lse[b, :, :t].double()
         assert torch.equal(torch.isnan(got), torch.isnan(o)), b
         fine = ~torch.isnan(o)
-        err, tol = (got - o).abs(), half_step(q.dtype) * o.abs() * 1.01 + (2 * ds + 2.0 ** -11 + 2.0 ** -16) * a + 2.0 ** -24
+        err, tol = (got - o).abs(), half_step(q.dtype) * o.abs() * 1.01 + (2 * ds + 2.0 ** -11 + 2.0 ** -16) * a + n * 2.0 ** -31 * big.unsqueeze(-1) + 2.0 ** -24
         assert bool((err[fine] <= tol[fine]).all()), (b, float((err[fine] / tol[fine]).max()))
         real = torch.isfinite(l)
         assert torch.equal(gl[~real & ~torch.isnan(l)], l[~real & ~torch.isnan(l)])
@@ -528,7 +531,7 @@ def test_a_run_of_all_of_them(elem, D, dtype):
         seen = torch.ones(T, n + T, dtype=torch.bool)
         seen[:, n:] = torch.ones(T, T).tril().bool() if mask is None else mask
         for b in range(B):
-            ref, _, a, _ = P.attention(q[b].to(dtype).double(), torch.cat((held[0][b], new[0][b]), 1), torch.cat((held[1][b], new[1][b]), 1), seen, D ** -0.5)
+            ref = P.attention(q[b].to(dtype).double(), torch.cat((held[0][b], new[0][b]), 1), torch.cat((held[1][b], new[1][b]), 1), seen, D ** -0.5)[0]
             # a norm that rounds the other way moves a key or a query by a step of its type, and an element of the cache by a step of its own
             step = {"e4m3": 2.0 ** -3, "e2m1": 2.0 ** -1}[elem]
             err = (o[b].cpu().double() - ref).norm() / ref.norm()

@@ -81,7 +81,7 @@ def _read():
 
 def _attention():
     from mpsa import serving
-    return serving._AttentionArgs(_cache(), ADDRESS, ADDRESS, None, ADDRESS, 1 << 40, *([128] * 6), 4, 0, ADDRESS, ADDRESS, None, None, 0, 1, 1, 4, 4, 0.1)
+    return serving._AttentionArgs(_cache(), ADDRESS, ADDRESS, None, ADDRESS, 1 << 40, *([128] * 6), 4, 0, ADDRESS, ADDRESS, None, None, ADDRESS, 0, 1, 1, 4, 4, 0.1)
 
 
 @pytest.mark.parametrize("make,name", [(_append, "mpsa_kv_append"), (_read, "mpsa_kv_read"), (_attention, "mpsa_kv_attention")])
@@ -104,7 +104,8 @@ def test_bad_caches_are_refused(make, name, change):
     (_attention, "mpsa_kv_attention", dict(Hq=3)), (_attention, "mpsa_kv_attention", dict(Hq=0)), (_attention, "mpsa_kv_attention", dict(B=70000)),
     (_attention, "mpsa_kv_attention", dict(sm_scale=0.0)), (_attention, "mpsa_kv_attention", dict(sm_scale=float("inf"))),
     (_attention, "mpsa_kv_attention", dict(sm_scale=float("nan"))), (_attention, "mpsa_kv_attention", dict(q_sl=4)),
-    (_attention, "mpsa_kv_attention", dict(out=ADDRESS + 2)), (_attention, "mpsa_kv_attention", dict(max_pages=-1)),
+    (_attention, "mpsa_kv_attention", dict(out=ADDRESS + 2)), (_attention, "mpsa_kv_attention", dict(max_pages=-1)), (_attention, "mpsa_kv_attention", dict(status=None)),
+    (_attention, "mpsa_kv_attention", dict(B=65535, max_pages=1 << 30)),
 ], ids=lambda v: str(v) if isinstance(v, dict) else None)
 def test_bad_arguments_are_refused(make, name, change):
     a = make()
