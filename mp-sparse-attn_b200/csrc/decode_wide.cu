@@ -1,16 +1,18 @@
 // Attention of many query rows over a paged MX cache (mpsa_kv_attention with more than 32 rows of a KV head: trees of drafted tokens, short
 // chunks) on the 5th-generation tensor cores.
 //
-// A unit is up to 128 query rows, a step 128 keys.  Nine warps: 4 convert, 4 are the softmax, one issues the tensor operations.
+// A unit is up to 128 query rows, a step 128 keys.  Eight warps: 4 are the softmax, 4 convert, the last of which also issues the tensor operations.
 //   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory.  K relative
 //             to the largest scale of its 32 keys (a factor of the scores), V relative to the largest of its key (a factor of P): what fp16
 //             cannot hold is 2^-30 of that.  Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an
 //             MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
-//   softmax   a thread a row: the row's reference U, set and raised as decode.cu says; P times V's factor, rounded to fp16, goes over S.
+//   softmax   a thread a row: the row's reference U, set and raised as decode.cu says; P times V's factor, rounded to fp16, goes over S.  Steps
+//             in which every row sees every key are tried against the references as they are, in one pass; where a product gets too large, and
+//             in the other steps, a pass over the scores finds the largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
 // One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
-// It is bound by the softmax warps' issue and the exponentials (16 a clock and SM, 1024 cycles a step).
+// It is bound by the issue of softmax and conversion together and by the exponentials (16 a clock and SM, 1024 cycles a step).
 #include "api_internal.h"
 #include "decode.cuh"
 
@@ -19,7 +21,7 @@
 namespace mpsa {
 namespace {
 
-constexpr int kThreads = 288, kColumns = 256;          // TMEM: S, over it P, then O from column 128
+constexpr int kThreads = 256, kColumns = 256;          // TMEM: S, over it P, then O from column 128
 constexpr float kMost = 15.0f, kSet = 7.0f;            // as in decode.cu
 constexpr int kLeast = -85;
 
@@ -28,8 +30,9 @@ struct Layout {
   static constexpr int half = 128 * 128;               // 64 depth elements of 128 rows
   static constexpr int tile = half * (D / 64);
   static constexpr int q = 0, k = tile, v = 2 * tile, vectors = 3 * tile;
-  // two steps' worth of: factors of P and log2 of them for 128 keys
-  static constexpr int bytes = vectors + 2 * 2 * 128 * 4 + 1024;       // (and what aligning the base may take)
+  // two steps' worth of: factors of P and log2 of them for 128 keys; then a converting warp's factors of its keys' blocks
+  static constexpr int factors = vectors + 2 * 2 * 128 * 4;
+  static constexpr int bytes = factors + 4 * 32 * 16 + 1024;           // (and what aligning the base may take)
 };
 
 struct Shared {
@@ -99,41 +102,62 @@ struct Run {
   int now;                                             // the sequence
 };
 
-// Keys on their way: a warp's 32 rows of K or V, and the scale codes of key `lane`
+// Keys on their way: a warp's 32 rows of K or V, and the scale codes of key `lane`.  A load takes rpi rows; which row and which 16 bytes a lane
+// has is chosen so that the lanes that store together meet different banks.
 template <int ELEM, int D>
 struct Rows {
-  static constexpr int row = code_bytes(ELEM, D), cpr = row / 16, rpi = 32 / cpr;       // 16-byte pieces of a row, rows of one load
+  static constexpr int row = code_bytes(ELEM, D), cpr = row / 16, rpi = 32 / cpr;
   uint4 code[cpr];
   uint32_t scale;
+  static __device__ __forceinline__ int piece(int lane) {
+    return cpr == 8 ? (lane & 3) | (lane >> 1 & 4) : cpr == 4 && ELEM == E2M1 ? (lane & 1) | (lane >> 2 & 2) : lane % cpr;
+  }
+  static __device__ __forceinline__ int key(int lane) {
+    return cpr == 8 ? (lane >> 2 & 1) | (lane >> 3 & 2) : cpr == 4 && ELEM == E2M1 ? (lane >> 1 & 3) | (lane >> 2 & 4) : lane / cpr;
+  }
 };
 
-// pos: the warp's first key; a lane's page is that of key pos + lane
+// Rows at the warp's 32 keys; at: row of key `lane` in the cache, -1 where there is none (16 keys lie side by side in a page)
 template <int ELEM, int D>
-__device__ __forceinline__ void request(Rows<ELEM, D>& r, const mpsa_kv_cache& c, const void* codes, const void* scales, int h, int pos, int page, bool there, int lane) {
+__device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, const void* scales, long long at, int keys, int lane) {
   using R = Rows<ELEM, D>;
-  const long long at = ((long long)max(page, 0) * c.Hkv + h) * c.page_size + ((pos + lane) & (c.page_size - 1));
   r.scale = 0;
-  if (there) r.scale = D == 128 ? static_cast<const uint32_t*>(scales)[at] : static_cast<const unsigned short*>(scales)[at];
+  if (at >= 0 && lane < keys) r.scale = D == 128 ? static_cast<const uint32_t*>(scales)[at] : static_cast<const unsigned short*>(scales)[at];
+  const int key = R::key(lane);
 #pragma unroll
-  for (int i = 0; i < R::cpr; ++i) {
-    const int key = i * R::rpi + lane / R::cpr;
-    const long long from = __shfl_sync(0xffffffffu, there ? at : -1ll, key);
-    r.code[i] = make_uint4(0, 0, 0, 0);
-    if (from >= 0) r.code[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(codes) + from * R::row + lane % R::cpr * 16);
+  for (int half = 0; half < 2; ++half) {
+    const long long base = __shfl_sync(0xffffffffu, at, 16 * half);
+    const uint8_t* const p = static_cast<const uint8_t*>(codes) + (base + key) * R::row + R::piece(lane) * 16;
+#pragma unroll
+    for (int i = 0; i < R::cpr / 2; ++i) {
+      uint4& c = r.code[half * (R::cpr / 2) + i];
+      c = make_uint4(0, 0, 0, 0);
+      if (base >= 0 && 16 * half + i * R::rpi + key < keys) c = *reinterpret_cast<const uint4*>(p + i * R::rpi * R::row);
+    }
   }
 }
 
-// fp16 rows into shared memory; `ref` (of lane's key) is subtracted from the scale codes; nan: what a NaN scale becomes
+// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by; base: of key `lane`, the
+// scale code that stands for 1; nan: what a NaN scale becomes.
 template <int ELEM, int D>
-__device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, int ref, uint32_t nan, int lane) {
+__device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, uint32_t factors, int base, uint32_t nan, int lane) {
   using R = Rows<ELEM, D>;
-  const int ch = lane % R::cpr, blk = ELEM == E2M1 ? ch : ch / 2;
+  constexpr int NB = D / 32;
+  uint32_t f[4] = {};
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const uint32_t e = r.scale >> (8 * i) & 255u;
+    f[i] = e == 255u ? nan : power2((int)e - base);
+  }
+  __syncwarp();
+  store_shared16(factors + 16 * lane, f[0], f[1], f[2], f[3]);
+  __syncwarp();
+  const int ch = R::piece(lane), blk = ELEM == E2M1 ? ch : ch / 2;
 #pragma unroll
   for (int i = 0; i < R::cpr; ++i) {
-    const int key = i * R::rpi + lane / R::cpr, row = row0 + key;
-    const uint32_t e = __shfl_sync(0xffffffffu, r.scale, key) >> (8 * blk) & 255u;
-    const int base = __shfl_sync(0xffffffffu, ref, key);
-    const uint32_t f = e == 255u ? nan : power2((int)e - base);
+    const int key = i * R::rpi + R::key(lane), row = row0 + key;
+    uint32_t m;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(m) : "r"(factors + 16 * key + 4 * blk) : "memory");
     const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
     if constexpr (ELEM == E2M1) {                      // 32 elements, 64 bytes
       const uint32_t to = tile + ch / 2 * (128 * 128) + row * 128;
@@ -141,23 +165,34 @@ __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, i
       for (int j = 0; j < 4; ++j) {
         uint32_t x[4];
         elem_quads(w[j], x[0], x[1], x[2], x[3]);
-        store_shared16(to + ((ch % 2 * 4 + j) ^ (row & 7)) * 16, times(x[0], f), times(x[1], f), times(x[2], f), times(x[3], f));
+        store_shared16(to + ((ch % 2 * 4 + j) ^ (row & 7)) * 16, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
       }
-    } else {                                           // 16 elements, 32 bytes; lanes of the upper half of the depth write their second piece first
+    } else {                                           // 16 elements, 32 bytes
       const uint32_t to = tile + ch / 4 * (128 * 128) + row * 128;
-      uint32_t x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        elem_two<ELEM>(w[j], x[2 * j], x[2 * j + 1]);
-        x[2 * j] = times(x[2 * j], f);
-        x[2 * j + 1] = times(x[2 * j + 1], f);
+      for (int j = 0; j < 2; ++j) {
+        uint32_t x[4];
+        elem_two<ELEM>(w[2 * j], x[0], x[1]);
+        elem_two<ELEM>(w[2 * j + 1], x[2], x[3]);
+        store_shared16(to + ((ch % 4 * 2 + j) ^ (row & 7)) * 16, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
       }
-      const bool late = D == 128 && ch >= 4;
-      const int c0 = ch % 4 * 2 + late, c1 = ch % 4 * 2 + !late;
-      store_shared16(to + (c0 ^ (row & 7)) * 16, late ? x[4] : x[0], late ? x[5] : x[1], late ? x[6] : x[2], late ? x[7] : x[3]);
-      store_shared16(to + (c1 ^ (row & 7)) * 16, late ? x[0] : x[4], late ? x[1] : x[5], late ? x[2] : x[6], late ? x[3] : x[7]);
     }
   }
+}
+
+// Which of the 32 keys from j0 on (counted among the query tokens) token `tok` sees.
+__device__ uint32_t seen_keys(const unsigned char* mask, int j0, int tok, int ql) {
+  const uint32_t before = j0 >= 0 ? 0u : j0 <= -32 ? ~0u : ~0u >> (32 + j0);           // bits below -j0: cached before the query tokens
+  if (tok >= ql || j0 <= -32) return before;
+  const int n = min((mask ? ql : tok + 1) - j0, 32);                                   // bits below n can be set
+  if (n <= 0) return before;
+  const uint32_t range = (~0u >> (32 - n)) & ~before;
+  if (!mask) return before | range;
+  uint32_t v = 0;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i)
+    if (range >> i & 1) v |= (uint32_t)(mask[j0 + i] != 0) << i;
+  return before | v;
 }
 
 template <typename T, int ELEM, int D>
@@ -172,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
   const int G = a.Hq / a.cache.Hkv, R = a.T * G;
 
   grid_dependents_go();
-  if (warp == 8) {
+  if (warp == 7) {
     tmem_alloc(&sh.tmem, kColumns);
     if (lane == 0) {
       mbar_init(&sh.k_full, 128);
@@ -246,80 +281,105 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         if (busy) {
           const bool special = pos + kWideStep > (a.T > 1 || a.mask ? run.first : run.len) ||
                                (sh.there[par][0] & sh.there[par][1] & sh.there[par][2] & sh.there[par][3]) != 0xffffffffu;
-          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};      // keys that this row sees
-          if (special) {
-            const unsigned char* const mk = a.mask + run.now * a.mask_sb + (long long)tok * a.T;
+          bool done = false;
+          if (!special && __all_sync(0xffffffffu, U != -INFINITY)) {
+            // as it is: products in registers, and over S if none has become too large
+            uint32_t p[64], top = 0;
+            float sum = 0.0f, sum2 = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              uint32_t v = 0;
-              for (int i = 0; i < 32; ++i) {
-                const int j = pos + 32 * c + i - run.first;
-                const bool seen = j < 0 || (live && tok < run.ql && j < run.ql && (a.mask ? mk[j] != 0 : j <= tok));
-                v |= (uint32_t)seen << i;
+              uint32_t x[32];
+              tmem_ld32(mine + 32 * c, x);
+              const float f = rs * sh.k_size[par][c];
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 z = *reinterpret_cast<const float4*>(vf + 32 * c + i);
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -U));
+                sum += y[0] + y[1];
+                sum2 += y[2] + y[3];
+                p[16 * c + i / 2] = pack2(__half(), y[0] * z.x, y[1] * z.y);
+                p[16 * c + i / 2 + 1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
+                top = __vmaxu2(top, __vmaxu2(p[16 * c + i / 2], p[16 * c + i / 2 + 1]));
               }
-              vis[c] = v & sh.there[par][c];
+            }
+            const float now = l + (sum + sum2);
+            // (a product of more than 2^15 is 0x7801 or more, an infinity or a NaN among them; a product cannot be negative)
+            done = !__any_sync(0xffffffffu, __vcmpgtu2(top, 0x78007800u) != 0 || !(now < 0x1p115f));
+            if (done) {
+              l = now;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = p[16 * c + i];
+                tmem_st16(mine + 16 * c, w);
+              }
             }
           }
-          float f[4];
+          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};      // keys that this row sees
+          if (!__all_sync(0xffffffffu, done)) {
+            if (special) {
+              const unsigned char* const mk = a.mask ? a.mask + run.now * a.mask_sb + (long long)min(tok, a.T - 1) * a.T : nullptr;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) f[c] = rs * sh.k_size[par][c];
-          // the largest product
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32];
-            tmem_ld32(mine + 32 * c, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 z = *reinterpret_cast<const float4*>(vl + 32 * c + i);
-              float y[4] = {fmaf(__uint_as_float(x[i]), f[c], z.x), fmaf(__uint_as_float(x[i + 1]), f[c], z.y), fmaf(__uint_as_float(x[i + 2]), f[c], z.z),
-                            fmaf(__uint_as_float(x[i + 3]), f[c], z.w)};
-              if (special)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (!(vis[c] >> (i + e) & 1)) y[e] = -INFINITY;
-              top = fmaxf(top, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+              for (int c = 0; c < 4; ++c) vis[c] = seen_keys(mk, pos + 32 * c - run.first, live ? tok : a.T, run.ql) & sh.there[par][c];
             }
-          }
-          const bool raise = top > U + kMost;
-          if (__any_sync(0xffffffffu, raise)) {
-            const float up = raise ? top - kSet : U, w = raise ? exp2_fast(U - up) : 1.0f;
-            if (__any_sync(0xffffffffu, raise && U != -INFINITY)) {   // (P V of the step before is over: Q K^T was issued behind it)
+            // the largest product
+            float top = -INFINITY;
 #pragma unroll 1
-              for (int i = 0; i < D / 16; ++i) {
-                uint32_t x[16];
-                tmem_ld16(mine + 128 + 16 * i, x);
-                tmem_ld_wait();
+            for (int c = 0; c < 4; ++c) {
+              uint32_t x[32];
+              tmem_ld32(mine + 32 * c, x);
+              const float f = rs * sh.k_size[par][c];
+              const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+              tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * w);
-                tmem_st16(mine + 128 + 16 * i, x);
+              for (int i = 0; i < 32; ++i) {
+                const float y = fmaf(__uint_as_float(x[i]), f, vl[32 * c + i]);
+                top = fmaxf(top, seen >> i & 1 ? y : -INFINITY);
               }
             }
-            l *= w;
-            U = up;
-          }
-          const float ref = U == -INFINITY ? 0.0f : U;
-          // P times V's factors over S: columns 16c .. of the 32c .. that have been read
+            const bool raise = top > U + kMost;
+            if (__any_sync(0xffffffffu, raise)) {
+              const float up = raise ? top - kSet : U, w = raise ? exp2_fast(U - up) : 1.0f;
+              if (__any_sync(0xffffffffu, raise && U != -INFINITY)) { // (P V of the step before is over: Q K^T was issued behind it)
+#pragma unroll 1
+                for (int i = 0; i < D / 16; ++i) {
+                  uint32_t x[16];
+                  tmem_ld16(mine + 128 + 16 * i, x);
+                  tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32], p[16];
-            tmem_ld32(mine + 32 * c, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 z = *reinterpret_cast<const float4*>(vf + 32 * c + i);
-              float y[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f[c], -ref));
-                if (special && !(vis[c] >> (i + e) & 1)) y[e] = 0.0f;
+                  for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * w);
+                  tmem_st16(mine + 128 + 16 * i, x);
+                }
               }
-              l += (y[0] + y[1]) + (y[2] + y[3]);
-              p[i / 2] = pack2(__half(), y[0] * z.x, y[1] * z.y);
-              p[i / 2 + 1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
+              l *= w;
+              U = up;
             }
-            tmem_st16(mine + 16 * c, p);
+            const float ref = U == -INFINITY ? 0.0f : U;
+            // P times V's factors over S: columns 16c .. of the 32c .. that have been read
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t x[32], p[16];
+              tmem_ld32(mine + 32 * c, x);
+              const float f = rs * sh.k_size[par][c];
+              const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float y[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -ref));
+                  if (!(seen >> (i + e) & 1)) y[e] = 0.0f;
+                }
+                l += y[0] + y[1];
+                p[i / 2] = pack2(__half(), y[0] * vf[32 * c + i], y[1] * vf[32 * c + i + 1]);
+              }
+              tmem_st16(mine + 16 * c, p);
+            }
           }
           // a value that is NaN: its block of the depth is, in the rows that see it
           uint32_t any = 0;
@@ -379,51 +439,60 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         else if (a.lse) static_cast<float*>(a.lse)[((long long)run.now * a.Hq + hq) * a.T + tok] = none ? -INFINITY : U + log2f(l);
       }
     }
-  } else if (warp < 8) {
-    // ---- conversion: keys 32 (warp - 4) .. of every step
-    const int w = warp - 4;
+  } else {
+    // ---- conversion: keys 32 (warp - 4) .. of every step; warp 7 issues the tensor operations too
+    constexpr uint32_t kQk = idesc_f16(0, 0, 128, 128), kPv = idesc_f16(0, 0, 128, D) | 1u << 16;     // (bit 16: B is MN-major)
+    const uint32_t qt = smem_u32(smem + Y::q), kt = smem_u32(smem + Y::k), vt = smem_u32(smem + Y::v);
+    const int w = warp - 4, shift = __popc(a.cache.page_size - 1);
+    const uint32_t factors = smem_u32(smem + Y::factors) + w * (32 * 16);
     const mpsa_kv_cache& c = a.cache;
     Rows<ELEM, D> k, v;
     Run ahead = run;                                   // one step ahead of `run`: what is requested
     bool more = ahead.next(a);
-    int as = more ? ahead.s0 : 0, page = -1, pos = 0;
-    bool there = false;
+    int as = more ? ahead.s0 : 0, keys = 0;
+    long long at = -1;
     auto look_up = [&]() {                             // the next step's keys
-      pos = kWideStep * as + 32 * w;
-      page = more ? page_of(a.page_table + ahead.now * a.table_sb, (pos + lane) / c.page_size, a.max_pages, c.num_pages) : -1;
-      there = page >= 0 && pos + lane < ahead.len;
+      const int pos = kWideStep * as + 32 * w;
+      const int page = more ? page_of(a.page_table + ahead.now * a.table_sb, (pos + lane) >> shift, a.max_pages, c.num_pages) : -1;
+      at = page < 0 ? -1 : (((long long)page * c.Hkv + ahead.h) << shift) + ((pos + lane) & (c.page_size - 1));
+      keys = ahead.len - pos;
+    };
+    auto pv = [&](uint32_t n) {                        // warp 7: P V of step n
+      if (!mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) || !mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mma_f16_ts(tmem + 128, tmem + 8 * i, make_sdesc(vt + i * 2048, Y::half, 1024, kLayoutSw128), kPv, 1);
+        tc_commit(&sh.pv_done);
+      }
+      __syncwarp();
+      return true;
     };
     look_up();
-    request<ELEM, D>(k, c, c.k, c.k_scale, ahead.h, pos, page, there, lane);
-    request<ELEM, D>(v, c, c.v, c.v_scale, ahead.h, pos, page, there, lane);
-    while (ok && run.next(a))
+    request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
+    request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
+    for (; ok && run.next(a); ++units)
       for (int s = run.s0; s < run.s1; ++s, ++n) {
         const int par = n & 1;
-        const bool here = there;
+        const bool here = at >= 0 && lane < keys;
         if (more && ++as == ahead.s1) {                // what comes after this step
           more = ahead.next(a);
           as = more ? ahead.s0 : 0;
         }
         look_up();
         if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
-        // K: one reference for the warp's keys
-        uint32_t top = 0;
+        // K: one reference for the warp's keys; V: one for each key
+        uint32_t top = 0, vtop = 0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const uint32_t e = k.scale >> (8 * i) & 255u;
+          const uint32_t e = k.scale >> (8 * i) & 255u, d = v.scale >> (8 * i) & 255u;
           top = max(top, e == 255u ? 0u : e);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        convert<ELEM, D>(k, smem_u32(smem + Y::k), 32 * w, (int)top, 0x7fff7fffu, lane);
-        // V: one for each key
-        uint32_t vtop = 0;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const uint32_t e = v.scale >> (8 * i) & 255u;
-          vtop = max(vtop, e == 255u ? 0u : e);
-          const uint32_t strange = __ballot_sync(0xffffffffu, e == 255u);
+          vtop = max(vtop, d == 255u ? 0u : d);
+          const uint32_t strange = __ballot_sync(0xffffffffu, d == 255u);
           if (lane == 0) sh.strange[par][w][i] = strange;
         }
+        top = __reduce_max_sync(0xffffffffu, top);
+        convert<ELEM, D>(k, kt, 32 * w, factors, (int)top, 0x7fff7fffu, lane);
         vectors[par * 256 + 32 * w + lane] = scale_value(vtop);
         vectors[par * 256 + 128 + 32 * w + lane] = (float)max((int)vtop - 127, kLeast);
         const uint32_t has = __ballot_sync(0xffffffffu, here);
@@ -433,54 +502,43 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         }
         fence_proxy_async_smem();
         mbar_arrive(&sh.k_full);
-        request<ELEM, D>(k, c, c.k, c.k_scale, ahead.h, pos, page, there, lane);
-        if (n > 0 && !(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;     // V is free
-        convert<ELEM, D>(v, smem_u32(smem + Y::v), 32 * w, (int)vtop, 0u, lane);
+        request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
+        if (n > 0) {
+          if (warp == 7 && !(ok = pv(n - 1))) break;
+          if (!(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;            // V and S, where P was, are free
+        }
+        if (warp == 7) {
+          ok = (s > run.s0 || mbar_wait(&sh.q_full, units & 1, a.status, KS_TIMEOUT_PIPE)) && mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              mma_f16_ss(tmem, sdesc_kmajor_sw128(qt + i / 4 * Y::half + i % 4 * 32), sdesc_kmajor_sw128(kt + i / 4 * Y::half + i % 4 * 32), kQk, i > 0);
+            tc_commit(&sh.s_full);
+          }
+          __syncwarp();
+        }
+        convert<ELEM, D>(v, vt, 32 * w, factors, (int)vtop, 0u, lane);
         fence_proxy_async_smem();
         mbar_arrive(&sh.v_full);
-        request<ELEM, D>(v, c, c.v, c.v_scale, ahead.h, pos, page, there, lane);
+        request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
       }
-  } else {
-    // ---- tensor operations
-    constexpr uint32_t kQk = idesc_f16(0, 0, 128, 128), kPv = idesc_f16(0, 0, 128, D) | 1u << 16;     // (bit 16: B is MN-major)
-    const uint32_t q = smem_u32(smem + Y::q), k = smem_u32(smem + Y::k), v = smem_u32(smem + Y::v);
-    for (; ok && run.next(a); ++units) {
-      ok = mbar_wait(&sh.q_full, units & 1, a.status, KS_TIMEOUT_PIPE);
-      for (int s = run.s0; ok && s < run.s1; ++s, ++n) {
-        // S is free when P V of the step before has read P
-        ok = mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE) && (n == 0 || mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA));
-        if (!ok) break;
-        tc_fence_after();
+    if (warp == 7) {
+      if (ok && n > 0) ok = pv(n - 1);
+      if (!ok) {                                       // what has been issued ends before its memory goes
         if (elect_one()) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            mma_f16_ss(tmem, sdesc_kmajor_sw128(q + i / 4 * Y::half + i % 4 * 32), sdesc_kmajor_sw128(k + i / 4 * Y::half + i % 4 * 32), kQk, i > 0);
-          tc_commit(&sh.s_full);
-        }
-        __syncwarp();
-        ok = mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) && mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mma_f16_ts(tmem + 128, tmem + 8 * i, make_sdesc(v + i * 2048, Y::half, 1024, kLayoutSw128), kPv, 1);
-          tc_commit(&sh.pv_done);
+          tc_commit(&sh.drained);
+          mbar_drain(&sh.drained, 0);
         }
         __syncwarp();
       }
-    }
-    if (!ok) {                                         // what has been issued ends before its memory goes
-      if (elect_one()) {
-        tc_commit(&sh.drained);
-        mbar_drain(&sh.drained, 0);
-      }
-      __syncwarp();
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, kColumns);
+  if (warp == 7) tmem_dealloc(tmem, kColumns);
 }
 
 template <typename T, int ELEM, int D>
