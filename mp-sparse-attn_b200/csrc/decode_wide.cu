@@ -117,22 +117,33 @@ struct Rows {
   }
 };
 
-// Rows at the warp's 32 keys; at: row of key `lane` in the cache, -1 where there is none (16 keys lie side by side in a page)
+// 16 bytes, or zeros: one predicated load.  (Written in C++ it becomes a choice between the loaded value and zero, which waits for the load.)
+__device__ __forceinline__ void load16(uint4& r, const void* p, bool there) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+               "@p ld.global.v4.b32 {%0,%1,%2,%3}, [%4];\n\t}" : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p), "r"((uint32_t)there) : "memory");
+}
+
+// Rows at the warp's 32 keys; at: row of key `lane` in the cache (fewer than 2^32 fit the memory), kNone where there is none (16 keys lie side
+// by side in a page)
+constexpr uint32_t kNone = ~0u;
 template <int ELEM, int D>
-__device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, const void* scales, long long at, int keys, int lane) {
+__device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, const void* scales, uint32_t at, int keys, int lane) {
   using R = Rows<ELEM, D>;
-  r.scale = 0;
-  if (at >= 0 && lane < keys) r.scale = D == 128 ? static_cast<const uint32_t*>(scales)[at] : static_cast<const unsigned short*>(scales)[at];
+  const uint32_t there = at != kNone && lane < keys;
+  if constexpr (D == 128)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(r.scale)
+                 : "l"(static_cast<const uint32_t*>(scales) + at), "r"(there) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}" : "=&r"(r.scale)
+                 : "l"(static_cast<const unsigned short*>(scales) + at), "r"(there) : "memory");
   const int key = R::key(lane);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const long long base = __shfl_sync(0xffffffffu, at, 16 * half);
-    const uint8_t* const p = static_cast<const uint8_t*>(codes) + (base + key) * R::row + R::piece(lane) * 16;
+    const uint32_t base = __shfl_sync(0xffffffffu, at, 16 * half);
+    const uint8_t* const p = static_cast<const uint8_t*>(codes) + ((unsigned long long)base + key) * R::row + R::piece(lane) * 16;
 #pragma unroll
     for (int i = 0; i < R::cpr / 2; ++i) {
-      uint4& c = r.code[half * (R::cpr / 2) + i];
-      c = make_uint4(0, 0, 0, 0);
-      if (base >= 0 && 16 * half + i * R::rpi + key < keys) c = *reinterpret_cast<const uint4*>(p + i * R::rpi * R::row);
+      load16(r.code[half * (R::cpr / 2) + i], p + i * R::rpi * R::row, base != kNone && 16 * half + i * R::rpi + key < keys);
     }
   }
 }
@@ -300,9 +311,10 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                 for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -U));
                 sum += y[0] + y[1];
                 sum2 += y[2] + y[3];
-                p[16 * c + i / 2] = pack2(__half(), y[0] * z.x, y[1] * z.y);
-                p[16 * c + i / 2 + 1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
-                top = __vmaxu2(top, __vmaxu2(p[16 * c + i / 2], p[16 * c + i / 2 + 1]));
+                uint32_t* const q = p + 16 * c + i / 2;
+                q[0] = pack2(__half(), y[0] * z.x, y[1] * z.y);
+                q[1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
+                top = __vmaxu2(top, __vmaxu2(q[0], q[1]));
               }
             }
             const float now = l + (sum + sum2);
@@ -447,15 +459,19 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
     const uint32_t factors = smem_u32(smem + Y::factors) + w * (32 * 16);
     const mpsa_kv_cache& c = a.cache;
     Rows<ELEM, D> k, v;
-    Run ahead = run;                                   // one step ahead of `run`: what is requested
-    bool more = ahead.next(a);
-    int as = more ? ahead.s0 : 0, keys = 0;
-    long long at = -1;
-    auto look_up = [&]() {                             // the next step's keys
+    bool more = run.next(a), opens = true;             // `run` is one step ahead, at what is requested; opens: the step is its part's first
+    int as = more ? run.s0 : 0, keys = 0;
+    uint32_t at = kNone;
+    // the table's entry for this lane's key of step `as`, and the one after, which is asked for a step early
+    auto entry_of = [&](int step) {
+      const int e = (kWideStep * step + 32 * w + lane) >> shift;
+      return more && step < run.s1 && e < a.max_pages ? a.page_table[run.now * a.table_sb + e] : -1;
+    };
+    int entry = entry_of(as), after = entry_of(as + 1);
+    auto look_up = [&]() {
       const int pos = kWideStep * as + 32 * w;
-      const int page = more ? page_of(a.page_table + ahead.now * a.table_sb, (pos + lane) >> shift, a.max_pages, c.num_pages) : -1;
-      at = page < 0 ? -1 : (((long long)page * c.Hkv + ahead.h) << shift) + ((pos + lane) & (c.page_size - 1));
-      keys = ahead.len - pos;
+      at = (unsigned)entry < (unsigned)c.num_pages ? (((uint32_t)entry * c.Hkv + run.h) << shift) + ((pos + lane) & (c.page_size - 1)) : kNone;
+      keys = run.len - pos;
     };
     auto pv = [&](uint32_t n) {                        // warp 7: P V of step n
       if (!mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) || !mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE)) return false;
@@ -471,14 +487,19 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
     look_up();
     request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
     request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
-    for (; ok && run.next(a); ++units)
-      for (int s = run.s0; s < run.s1; ++s, ++n) {
+    for (bool have = more; have; ++n) {
         const int par = n & 1;
-        const bool here = at >= 0 && lane < keys;
-        if (more && ++as == ahead.s1) {                // what comes after this step
-          more = ahead.next(a);
-          as = more ? ahead.s0 : 0;
+        const bool here = at != kNone && lane < keys, first = opens;
+        opens = false;
+        if (++as == run.s1) {                          // what comes after this step
+          more = run.next(a);
+          as = more ? run.s0 : 0;
+          after = entry_of(as);
+          opens = true;
         }
+        have = more;
+        entry = after;
+        after = entry_of(as + 1);
         look_up();
         if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
         // K: one reference for the warp's keys; V: one for each key
@@ -508,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
           if (!(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;            // V and S, where P was, are free
         }
         if (warp == 7) {
-          ok = (s > run.s0 || mbar_wait(&sh.q_full, units & 1, a.status, KS_TIMEOUT_PIPE)) && mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE);
+          ok = (!first || mbar_wait(&sh.q_full, units++ & 1, a.status, KS_TIMEOUT_PIPE)) && mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
