@@ -1,15 +1,16 @@
 // Attention of many query rows over a paged MX cache (mpsa_kv_attention with more than 32 rows of a KV head: trees of drafted tokens, short
 // chunks) on the 5th-generation tensor cores.
 //
-// A unit is up to 128 query rows, a step 128 keys.  Eight warps: 4 are the softmax, 4 convert, the last of which also issues the tensor operations.
-//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory.  K relative
-//             to the largest scale of its 32 keys (a factor of the scores), V relative to the largest of its key (a factor of P): what fp16
-//             cannot hold is 2^-30 of that.  Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an
-//             MN-major one.
+// A unit is up to 128 query rows, a step 128 keys.  Eight warps: 4 convert, 4 are the softmax, the first of which also issues the
+// tensor operations: what they wait for is what it has just done.
+//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory, relative to
+//             the largest scale of 32 keys of K or of V: what fp16 cannot hold is 2^-30 of the largest of those elements, E2M1 apart even less.
+//             Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
-//   softmax   a thread a row: the row's reference U, set and raised as decode.cu says; P times V's factor, rounded to fp16, goes over S.  Steps
-//             in which every row sees every key are tried against the references as they are, in one pass; where a product gets too large, and
-//             in the other steps, a pass over the scores finds the largest one first.
+//   softmax   a thread a row: P times the largest scale of V of the 32 keys, rounded to fp16, goes over S; the reference U keeps that within
+//             fp16 as decode.cu says (there it is each block's own scale).  Steps in which every row sees every key are tried against the
+//             references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
+//             largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
 // One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
 // It is bound by the issue of softmax and conversion together and by the exponentials (16 a clock and SM, 1024 cycles a step).
@@ -23,22 +24,21 @@ namespace {
 
 constexpr int kThreads = 256, kColumns = 256;          // TMEM: S, over it P, then O from column 128
 constexpr float kMost = 15.0f, kSet = 7.0f;            // as in decode.cu
-constexpr int kLeast = -85;
+constexpr float kLeast = -85.0f;
 
 template <int D>
 struct Layout {
   static constexpr int half = 128 * 128;               // 64 depth elements of 128 rows
   static constexpr int tile = half * (D / 64);
-  static constexpr int q = 0, k = tile, v = 2 * tile, vectors = 3 * tile;
-  // two steps' worth of: factors of P and log2 of them for 128 keys; then a converting warp's factors of its keys' blocks
-  static constexpr int factors = vectors + 2 * 2 * 128 * 4;
+  static constexpr int q = 0, k = tile, v = 2 * tile;
+  static constexpr int factors = 3 * tile;             // a converting warp's factors of its keys' blocks
   static constexpr int bytes = factors + 4 * 32 * 16 + 1024;           // (and what aligning the base may take)
 };
 
 struct Shared {
   uint64_t k_full, v_full, s_full, p_full, pv_done, q_full, drained;
   uint32_t tmem;
-  float k_size[2][4];                                  // 2^(largest scale of 32 keys)
+  float k_size[2][4], v_size[2][4];                    // largest scale of 32 keys: of K, log2 of V's (two steps' worth, as below)
   uint32_t there[2][4];                                // keys with a page and within the length
   uint32_t strange[2][4][4];                           // [32 keys][block of the depth]: scales of V that are NaN
 };
@@ -148,8 +148,8 @@ __device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, con
   }
 }
 
-// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by; base: of key `lane`, the
-// scale code that stands for 1; nan: what a NaN scale becomes.
+// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by; base: the scale code that
+// stands for 1; nan: what a NaN scale becomes.
 template <int ELEM, int D>
 __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, uint32_t factors, int base, uint32_t nan, int lane) {
   using R = Rows<ELEM, D>;
@@ -163,30 +163,28 @@ __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, i
   __syncwarp();
   store_shared16(factors + 16 * lane, f[0], f[1], f[2], f[3]);
   __syncwarp();
-  const int ch = R::piece(lane), blk = ELEM == E2M1 ? ch : ch / 2;
+  // A row's 16-byte pieces lie exclusive-ored with the row's last three bits: for one lane the places of all its pieces differ from the first
+  // one's by bits that are known here (rows of one lane are rpi apart) and by whole rows.
+  const int ch = R::piece(lane), key = R::key(lane);
+  constexpr int out = ELEM == E2M1 ? 4 : 2;            // pieces that 16 bytes of codes become
+  constexpr int halves = 8 / out;                      // code pieces of 64 depth elements
+  const uint32_t first = tile + ch / halves * (128 * 128) + (row0 + key) * 128 + ((ch % halves * out) ^ (key & 7)) * 16;
+  const uint32_t mul = factors + 16 * key + 4 * (ELEM == E2M1 ? ch : ch / 2);
 #pragma unroll
   for (int i = 0; i < R::cpr; ++i) {
-    const int key = i * R::rpi + R::key(lane), row = row0 + key;
     uint32_t m;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(m) : "r"(factors + 16 * key + 4 * blk) : "memory");
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(m) : "r"(mul + i * R::rpi * 16) : "memory");
     const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
-    if constexpr (ELEM == E2M1) {                      // 32 elements, 64 bytes
-      const uint32_t to = tile + ch / 2 * (128 * 128) + row * 128;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t x[4];
+    for (int j = 0; j < out; ++j) {
+      uint32_t x[4];
+      if constexpr (ELEM == E2M1) {
         elem_quads(w[j], x[0], x[1], x[2], x[3]);
-        store_shared16(to + ((ch % 2 * 4 + j) ^ (row & 7)) * 16, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
-      }
-    } else {                                           // 16 elements, 32 bytes
-      const uint32_t to = tile + ch / 4 * (128 * 128) + row * 128;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t x[4];
+      } else {
         elem_two<ELEM>(w[2 * j], x[0], x[1]);
         elem_two<ELEM>(w[2 * j + 1], x[2], x[3]);
-        store_shared16(to + ((ch % 4 * 2 + j) ^ (row & 7)) * 16, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
       }
+      store_shared16((first ^ (16 * j + (R::rpi == 4 ? i % 2 * 64 : 0))) + i * R::rpi * 128, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
     }
   }
 }
@@ -213,7 +211,6 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
   extern __shared__ uint8_t raw[];
   __shared__ Shared sh;
   uint8_t* const smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  float* const vectors = reinterpret_cast<float*>(smem + Y::vectors);  // [parity][0: factor, 1: log2][key]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = a.Hq / a.cache.Hkv, R = a.T * G;
 
@@ -242,8 +239,34 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
   uint32_t units = 0;
   bool ok = true;
 
+  const uint32_t qt = smem_u32(smem + Y::q), kt = smem_u32(smem + Y::k), vt = smem_u32(smem + Y::v);
   if (warp < 4) {
-    // ---- softmax: row warp * 32 + lane of the unit
+    // ---- softmax: row warp * 32 + lane of the unit; warp 0 issues the tensor operations too
+    constexpr uint32_t kQk = idesc_f16(0, 0, 128, 128), kPv = idesc_f16(0, 0, 128, D) | 1u << 16;     // (bit 16: B is MN-major)
+    // Q K^T of step n.  (S, where P was, is free: P V of the step before has been waited for.)
+    auto qk = [&]() {
+      if (!mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          mma_f16_ss(tmem, sdesc_kmajor_sw128(qt + i / 4 * Y::half + i % 4 * 32), sdesc_kmajor_sw128(kt + i / 4 * Y::half + i % 4 * 32), kQk, i > 0);
+        tc_commit(&sh.s_full);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto pv = [&]() {
+      if (!mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) || !mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mma_f16_ts(tmem + 128, tmem + 8 * i, make_sdesc(vt + i * 2048, Y::half, 1024, kLayoutSw128), kPv, 1);
+        tc_commit(&sh.pv_done);
+      }
+      __syncwarp();
+      return true;
+    };
     const uint32_t mine = tmem + (uint32_t)(warp * 32) * 65536u;
     for (; ok && run.next(a); ++units) {
       const int r = run.row0 + warp * 32 + lane, tok = r / G, hq = run.h * G + r % G;
@@ -282,13 +305,13 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sh.q_full);
+        if (warp == 0) ok = mbar_wait(&sh.q_full, units & 1, a.status, KS_TIMEOUT_PIPE) && qk();
       }
       float U = -INFINITY, l = 0.0f;
-      for (int s = run.s0; s < run.s1; ++s, ++n) {
+      for (int s = run.s0; ok && s < run.s1; ++s) {
         if (!(ok = mbar_wait(&sh.s_full, n & 1, a.status, KS_TIMEOUT_MMA))) break;
         tc_fence_after();
         const int par = n & 1, pos = s * kWideStep;
-        const float *vf = vectors + par * 256, *vl = vf + 128;
         if (busy) {
           const bool special = pos + kWideStep > (a.T > 1 || a.mask ? run.first : run.len) ||
                                (sh.there[par][0] & sh.there[par][1] & sh.there[par][2] & sh.there[par][3]) != 0xffffffffu;
@@ -296,29 +319,29 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
           if (!special && __all_sync(0xffffffffu, U != -INFINITY)) {
             // as it is: products in registers, and over S if none has become too large
             uint32_t p[64], top = 0;
-            float sum = 0.0f, sum2 = 0.0f;
+            float now = l;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c];
+              const float f = rs * sh.k_size[par][c], v = sh.v_size[par][c], ref = v - U;
+              float sum = 0.0f, sum2 = 0.0f;
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                const float4 z = *reinterpret_cast<const float4*>(vf + 32 * c + i);
                 float y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -U));
+                for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, ref));
                 sum += y[0] + y[1];
                 sum2 += y[2] + y[3];
                 uint32_t* const q = p + 16 * c + i / 2;
-                q[0] = pack2(__half(), y[0] * z.x, y[1] * z.y);
-                q[1] = pack2(__half(), y[2] * z.z, y[3] * z.w);
+                q[0] = pack2(__half(), y[0], y[1]);
+                q[1] = pack2(__half(), y[2], y[3]);
                 top = __vmaxu2(top, __vmaxu2(q[0], q[1]));
               }
+              now = fmaf(sum + sum2, exp2_fast(-v), now);
             }
-            const float now = l + (sum + sum2);
-            // (a product of more than 2^15 is 0x7801 or more, an infinity or a NaN among them; a product cannot be negative)
+            // (a product of more than 2^15 is 0x7801 or more, an infinity or a NaN among them; none is negative)
             done = !__any_sync(0xffffffffu, __vcmpgtu2(top, 0x78007800u) != 0 || !(now < 0x1p115f));
             if (done) {
               l = now;
@@ -344,12 +367,12 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c];
+              const float f = rs * sh.k_size[par][c], v = fmaxf(sh.v_size[par][c], kLeast);
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float y = fmaf(__uint_as_float(x[i]), f, vl[32 * c + i]);
+                const float y = fmaf(__uint_as_float(x[i]), f, v);
                 top = fmaxf(top, seen >> i & 1 ? y : -INFINITY);
               }
             }
@@ -376,20 +399,22 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32], p[16];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c];
+              const float f = rs * sh.k_size[par][c], v = sh.v_size[par][c], at = v - ref;
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+              float sum = 0.0f;
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 float y[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -ref));
+                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, at));
                   if (!(seen >> (i + e) & 1)) y[e] = 0.0f;
                 }
-                l += y[0] + y[1];
-                p[i / 2] = pack2(__half(), y[0] * vf[32 * c + i], y[1] * vf[32 * c + i + 1]);
+                sum += y[0] + y[1];
+                p[i / 2] = pack2(__half(), y[0], y[1]);
               }
+              l = fmaf(sum, exp2_fast(-v), l);
               tmem_st16(mine + 16 * c, p);
             }
           }
@@ -421,6 +446,9 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         }
         tc_fence_before();
         mbar_arrive(&sh.p_full);
+        if (warp == 0 && !(ok = pv())) break;
+        ++n;
+        if (warp == 0 && s + 1 < run.s1) ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA) && qk();
       }
       if (!ok || !(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;
       tc_fence_after();
@@ -451,59 +479,65 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         else if (a.lse) static_cast<float*>(a.lse)[((long long)run.now * a.Hq + hq) * a.T + tok] = none ? -INFINITY : U + log2f(l);
       }
     }
+    if (warp == 0 && !ok) {                            // what has been issued ends before its memory goes
+      if (elect_one()) {
+        tc_commit(&sh.drained);
+        mbar_drain(&sh.drained, 0);
+      }
+      __syncwarp();
+    }
   } else {
-    // ---- conversion: keys 32 (warp - 4) .. of every step; warp 7 issues the tensor operations too
-    constexpr uint32_t kQk = idesc_f16(0, 0, 128, 128), kPv = idesc_f16(0, 0, 128, D) | 1u << 16;     // (bit 16: B is MN-major)
-    const uint32_t qt = smem_u32(smem + Y::q), kt = smem_u32(smem + Y::k), vt = smem_u32(smem + Y::v);
+    // ---- conversion: keys 32 (warp - 4) .. of every step
     const int w = warp - 4, shift = __popc(a.cache.page_size - 1);
     const uint32_t factors = smem_u32(smem + Y::factors) + w * (32 * 16);
     const mpsa_kv_cache& c = a.cache;
     Rows<ELEM, D> k, v;
-    bool more = run.next(a), opens = true;             // `run` is one step ahead, at what is requested; opens: the step is its part's first
+    bool more = run.next(a);                           // `run` is one step ahead, at what is requested
     int as = more ? run.s0 : 0, keys = 0;
     uint32_t at = kNone;
-    // the table's entry for this lane's key of step `as`, and the one after, which is asked for a step early
+    // the table's entries for this lane's key of step `as` and the two behind it: asked for two steps early, and the rows brought to L2 one step early
     auto entry_of = [&](int step) {
       const int e = (kWideStep * step + 32 * w + lane) >> shift;
-      return more && step < run.s1 && e < a.max_pages ? a.page_table[run.now * a.table_sb + e] : -1;
+      int r;
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, -1;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(r)
+                   : "l"(a.page_table + run.now * a.table_sb + e), "r"((uint32_t)(more && step < run.s1 && e < a.max_pages)) : "memory");
+      return r;
     };
-    int entry = entry_of(as), after = entry_of(as + 1);
+    int entry = -1, after = entry_of(as), later = entry_of(as + 1);
+    auto row_of = [&](int e, int pos) {
+      return (unsigned)e < (unsigned)c.num_pages ? (((uint32_t)e * c.Hkv + run.h) << shift) + ((pos + lane) & (c.page_size - 1)) : kNone;
+    };
     auto look_up = [&]() {
       const int pos = kWideStep * as + 32 * w;
-      at = (unsigned)entry < (unsigned)c.num_pages ? (((uint32_t)entry * c.Hkv + run.h) << shift) + ((pos + lane) & (c.page_size - 1)) : kNone;
+      at = row_of(entry, pos);
       keys = run.len - pos;
-    };
-    auto pv = [&](uint32_t n) {                        // warp 7: P V of step n
-      if (!mbar_wait(&sh.p_full, n & 1, a.status, KS_TIMEOUT_PIPE) || !mbar_wait(&sh.v_full, n & 1, a.status, KS_TIMEOUT_PIPE)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mma_f16_ts(tmem + 128, tmem + 8 * i, make_sdesc(vt + i * 2048, Y::half, 1024, kLayoutSw128), kPv, 1);
-        tc_commit(&sh.pv_done);
+      const uint32_t row = row_of(after, pos + kWideStep);
+      if (row != kNone && lane < keys - kWideStep) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(c.k) + (unsigned long long)row * code_bytes(ELEM, D)));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(c.v) + (unsigned long long)row * code_bytes(ELEM, D)));
       }
-      __syncwarp();
-      return true;
     };
-    look_up();
-    request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
-    request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
-    for (bool have = more; have; ++n) {
-        const int par = n & 1;
-        const bool here = at != kNone && lane < keys, first = opens;
-        opens = false;
-        if (++as == run.s1) {                          // what comes after this step
-          more = run.next(a);
-          as = more ? run.s0 : 0;
-          after = entry_of(as);
-          opens = true;
-        }
-        have = more;
-        entry = after;
-        after = entry_of(as + 1);
-        look_up();
+    // A turn converts a step (the first one none) and requests the one behind it.  Each operand is requested in one place: where two places
+    // meet, the loaded registers are copied, and a copy waits for the load.
+    for (bool have = false;;) {
+      const int par = n & 1;
+      const bool now = have, here = at != kNone && lane < keys;
+      if (now && ++as == run.s1) {
+        more = run.next(a);
+        as = more ? run.s0 : 0;
+        after = entry_of(as);
+        later = entry_of(as + 1);
+      }
+      uint32_t vtop = 0;
+      have = more;
+      entry = after;
+      after = later;
+      later = entry_of(as + 2);
+      look_up();
+      if (now) {
         if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
-        // K: one reference for the warp's keys; V: one for each key
-        uint32_t top = 0, vtop = 0;
+        // one reference for the warp's keys of K, and one for V
+        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const uint32_t e = k.scale >> (8 * i) & 255u, d = v.scale >> (8 * i) & 255u;
@@ -513,47 +547,27 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
           if (lane == 0) sh.strange[par][w][i] = strange;
         }
         top = __reduce_max_sync(0xffffffffu, top);
+        vtop = __reduce_max_sync(0xffffffffu, max(vtop, 1u));
         convert<ELEM, D>(k, kt, 32 * w, factors, (int)top, 0x7fff7fffu, lane);
-        vectors[par * 256 + 32 * w + lane] = scale_value(vtop);
-        vectors[par * 256 + 128 + 32 * w + lane] = (float)max((int)vtop - 127, kLeast);
         const uint32_t has = __ballot_sync(0xffffffffu, here);
         if (lane == 0) {
           sh.there[par][w] = has;
           sh.k_size[par][w] = scale_value(top);
+          sh.v_size[par][w] = (float)((int)vtop - 127);
         }
         fence_proxy_async_smem();
         mbar_arrive(&sh.k_full);
-        request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
-        if (n > 0) {
-          if (warp == 7 && !(ok = pv(n - 1))) break;
-          if (!(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;            // V and S, where P was, are free
-        }
-        if (warp == 7) {
-          ok = (!first || mbar_wait(&sh.q_full, units++ & 1, a.status, KS_TIMEOUT_PIPE)) && mbar_wait(&sh.k_full, n & 1, a.status, KS_TIMEOUT_PIPE);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-              mma_f16_ss(tmem, sdesc_kmajor_sw128(qt + i / 4 * Y::half + i % 4 * 32), sdesc_kmajor_sw128(kt + i / 4 * Y::half + i % 4 * 32), kQk, i > 0);
-            tc_commit(&sh.s_full);
-          }
-          __syncwarp();
-        }
+      }
+      request<ELEM, D>(k, c.k, c.k_scale, at, keys, lane);
+      if (now) {
+        if (n > 0 && !(ok = mbar_wait(&sh.pv_done, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;     // V is free
         convert<ELEM, D>(v, vt, 32 * w, factors, (int)vtop, 0u, lane);
         fence_proxy_async_smem();
         mbar_arrive(&sh.v_full);
-        request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
+        ++n;
       }
-    if (warp == 7) {
-      if (ok && n > 0) ok = pv(n - 1);
-      if (!ok) {                                       // what has been issued ends before its memory goes
-        if (elect_one()) {
-          tc_commit(&sh.drained);
-          mbar_drain(&sh.drained, 0);
-        }
-        __syncwarp();
-      }
+      if (!have) break;
+      request<ELEM, D>(v, c.v, c.v_scale, at, keys, lane);
     }
   }
   tc_fence_before();
