@@ -27,6 +27,7 @@ namespace mpsa {
 namespace {
 
 constexpr int kWarps = 4, kStep = 32;
+constexpr int kMostCluster = 8, kClusterSteps = 64;
 constexpr float kMost = 15.0f, kSet = 7.0f;    // log2 of the largest product that raises no reference, and of the largest one after a raise
 constexpr int kLeast = -85;                    // log2 of a scale that counts as that at least: references are the largest score - 100 at least
 
@@ -109,13 +110,45 @@ __device__ __forceinline__ void v_fragments(uint32_t p, uint32_t (&f)[ELEM == E2
     }
 }
 
-template <typename T, int ELEM, int D, int NR>
+// Cluster barrier: what its CTAs wrote to shared memory before it can be read by all of them after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t p) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_cluster2(uint32_t p) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p) : "memory");
+  return v;
+}
+
+// Four elements of a row's output.
+template <typename T>
+__device__ __forceinline__ void write_out(const Call& a, int b, int h, int G, int row, int ql, int d, float4 v, float top, float sum) {
+  const int tok = row / G, hq = h * G + row % G;
+  const bool none = sum == 0.0f || tok >= ql;
+  const float f = none ? 0.0f : 1.0f / sum;
+  const float y[4] = {none ? 0.0f : v.x * f, none ? 0.0f : v.y * f, none ? 0.0f : v.z * f, none ? 0.0f : v.w * f};
+  store4(static_cast<T*>(a.out) + (b * a.o_sb + hq * a.o_sh + (long long)tok * a.o_sl + d), y);
+  if (a.lse && d == 0) static_cast<float*>(a.lse)[((long long)b * a.Hq + hq) * a.T + tok] = none ? -INFINITY : top + log2f(sum);
+}
+
+// CLUSTER: a.cluster CTAs share a unit, each has an equal run of its steps, and they add up their parts through shared memory.
+template <typename T, int ELEM, int D, int NR, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != E2M1 ? 3 : 4) kv_attention_kernel(const __grid_constant__ Call a) {
   using Y = Layout<ELEM, D, NR>;
   constexpr int NB = D / 32, NM = kStep / 16;          // blocks of the depth, key tiles of a step
   constexpr int BP = ELEM == E2M1 ? 2 : 1;             // blocks of a 32-byte piece
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 row_stat[kWarps][8 * NR];
+  __shared__ float2 row_stat[kWarps][8 * NR], unit_stat[CLUSTER ? 8 * NR : 1];
   const mpsa_kv_cache& c = a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const uint32_t ring = smem_u32(smem) + warp * Y::warp;
@@ -127,14 +160,26 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
   const uint32_t mat = (lane & 15) * Y::row + ((lane >> 4) ^ Y::swap(lane & 15)) * 16;  // this lane's row address for ldmatrix
 
   grid_dependents_go();
-  uint32_t share, begin;
-  int b = locate(a, gridDim.x, blockIdx.x, share, begin, lane);
-  uint32_t at = blockIdx.x * share;
-  const uint32_t stop = at + min(share, ~at);
+  uint32_t share, begin = 0, at = 0, stop = 1;
+  int b = CLUSTER ? blockIdx.x / a.cluster / units : locate(a, gridDim.x, blockIdx.x, share, begin, lane);
+  if constexpr (!CLUSTER) {
+    at = blockIdx.x * share;
+    stop = at + min(share, ~at);
+  }
   for (bool again = false; b < a.B && at < stop; again = true) {
     const int len = length_of(a, b), steps = steps_of(a, len);
-    const uint32_t off = at - begin;
-    const int u = off / (uint32_t)steps, s0 = off - u * (uint32_t)steps, s1 = min((uint32_t)steps, s0 + (stop - at));
+    int u, s0, s1;
+    if constexpr (CLUSTER) {
+      const int rank = blockIdx.x % a.cluster, per = (steps + a.cluster - 1) / a.cluster;
+      u = blockIdx.x / a.cluster % units;
+      s0 = min(rank * per, steps);
+      s1 = min(s0 + per, steps);
+    } else {
+      const uint32_t off = at - begin;
+      u = off / (uint32_t)steps;
+      s0 = off - u * (uint32_t)steps;
+      s1 = min((uint32_t)steps, s0 + (stop - at));
+    }
     const int h = u / a.groups, row0 = u % a.groups * Y::rows;
     const int ql = queries_of(a, b, len), first = len - ql;
     const int* const table = a.page_table + b * a.table_sb;
@@ -471,20 +516,41 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
         sum += f * row_stat[w][r].y;
         v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
       }
-      if (whole) {
-        const int tok = (row0 + r) / G, hq = h * G + (row0 + r) % G;
-        const bool none = sum == 0.0f || tok >= ql;
-        const float f = none ? 0.0f : 1.0f / sum;
-        const float y[4] = {none ? 0.0f : v.x * f, none ? 0.0f : v.y * f, none ? 0.0f : v.z * f, none ? 0.0f : v.w * f};
-        store4(static_cast<T*>(a.out) + (b * a.o_sb + hq * a.o_sh + tok * a.o_sl + d), y);
-        if (a.lse && d == 0) static_cast<float*>(a.lse)[((long long)b * a.Hq + hq) * a.T + tok] = none ? -INFINITY : top + log2f(sum);
+      if constexpr (CLUSTER) {                        // (the place of warp 0's part: nobody else reads it)
+        *reinterpret_cast<float4*>(merge + r * Y::pitch + d) = v;
+        if (d == 0) unit_stat[r] = make_float2(top, sum);
+      } else if (whole) {
+        write_out<T>(a, b, h, G, row0 + r, ql, d, v, top, sum);
       } else {
         *reinterpret_cast<float4*>(a.part + (slot * Y::rows + r) * D + d) = v;
         if (d == 0) a.stat[slot * Y::rows + r] = make_float2(top, sum);
       }
     }
+    if constexpr (CLUSTER) {
+      cluster_sync();
+      const uint32_t parts = smem_u32(merge), stats = smem_u32(unit_stat);
+      for (int i = blockIdx.x % a.cluster * (32 * kWarps) + threadIdx.x; i < Y::rows * (D / 4); i += a.cluster * (32 * kWarps)) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        if (row0 + r >= R) continue;
+        float top = -INFINITY, sum = 0.0f;
+        for (int c = 0; c < a.cluster; ++c) top = fmaxf(top, load_cluster2(at_rank(stats + r * 8, c)).x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (int c = 0; c < a.cluster; ++c) {
+          const float2 st = load_cluster2(at_rank(stats + r * 8, c));
+          const float4 y = load_cluster4(at_rank(parts + (r * Y::pitch + d) * 4, c));
+          const float f = exp2_fast(st.x - ref);
+          sum += f * st.y;
+          v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
+        }
+        write_out<T>(a, b, h, G, row0 + r, ql, d, v, top, sum);
+      }
+      cluster_sync();                                 // (nobody's shared memory goes before all have read it)
+      return;
+    }
     at += s1 - s0;
-    if (at - begin >= (uint32_t)steps * units) {
+    if (!CLUSTER && at - begin >= (uint32_t)steps * units) {
       begin += (uint32_t)steps * units;
       ++b;
     }
@@ -564,8 +630,28 @@ template <typename T, int ELEM, int D, int NR>
 int launch(const Call& a, int ctas, cudaStream_t st) {
   constexpr int bytes = Layout<ELEM, D, NR>::bytes;
   constexpr int id = (std::is_same_v<T, __half> ? 10000 : 0) + ELEM * 1000 + D * 8 + NR;
-  if (!allow_smem<id>(kv_attention_kernel<T, ELEM, D, NR>, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-  kv_attention_kernel<T, ELEM, D, NR><<<ctas, 32 * kWarps, bytes, st>>>(a);
+  if constexpr (NR <= 2) {
+    if (a.cluster) {
+      const auto kernel = kv_attention_kernel<T, ELEM, D, NR, true>;
+      if (!allow_smem<20000 + id>(kernel, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(a.B * a.cache.Hkv * a.groups * a.cluster);
+      cfg.blockDim = dim3(32 * kWarps);
+      cfg.dynamicSmemBytes = bytes;
+      cfg.stream = st;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = a.cluster;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      cudaLaunchKernelEx(&cfg, kernel, a);
+      return check_launch("kv_attention");
+    }
+  }
+  const auto kernel = kv_attention_kernel<T, ELEM, D, NR, false>;
+  if (!allow_smem<id>(kernel, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
+  kernel<<<ctas, 32 * kWarps, bytes, st>>>(a);
   return check_launch("kv_attention");
 }
 template <typename T, int ELEM, int D>
@@ -582,11 +668,22 @@ int launch_all(const Call& a, cudaStream_t st) {
   if (int rc = wide(a) ? launch_wide(a, ctas, st)
                        : elem == E4M3 ? launch_depth<T, E4M3>(a, ctas, st) : elem == E5M2 ? launch_depth<T, E5M2>(a, ctas, st) : launch_depth<T, E2M1>(a, ctas, st))
     return rc;
+  if (a.cluster) return MPSA_OK;
   const int rows = a.T * (a.Hq / a.cache.Hkv);
   const dim3 grid(a.B * a.cache.Hkv * a.groups, (std::min(rows, a.rows) + kWarps - 1) / kWarps);
   if (a.cache.D == 64) launch_dependent(kv_combine_kernel<T, 64>, grid, 32 * kWarps, 0, st, true, a, ctas);
   else launch_dependent(kv_combine_kernel<T, 128>, grid, 32 * kWarps, 0, st, true, a, ctas);
   return check_launch("kv_attention");
+}
+
+// CTAs of a cluster for each unit, or 0 for runs and the combining launch.  Clusters where the table holds so little that a unit's steps keep
+// few warps busy for a short time: then the combining launch costs more than what equal runs gain with uneven lengths.
+int cluster_of(const Call& a) {
+  if (a.rows > 16) return 0;
+  const double units = (double)a.B * a.cache.Hkv * a.groups, room = 3.0 * sm_count(), steps = (double)a.max_pages * a.cache.page_size / a.step;
+  int c = 1;
+  while (c < kMostCluster && units * 2 * c <= room && steps > 4 * c) c *= 2;
+  return steps <= (double)kClusterSteps * c && units * c <= 65535.0 * 16 ? c : 0;
 }
 
 // The call with its plan and its workspace's parts; the workspace's bytes, or an error.
@@ -605,12 +702,13 @@ long long plan(const mpsa_kv_attention_args* args, Call& a) {
   a.step = wide(a) ? kWideStep : kStep;
   a.least = wide(a) ? 2 : 4;                          // (four: a step for each warp)
   a.groups = (rows + a.rows - 1) / a.rows;
+  a.cluster = cluster_of(a);
   const double most = (double)a.B * a.cache.Hkv * a.groups * ((double)a.max_pages * a.cache.page_size / a.step + 1);
   if (most > 4e9) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: sequences x heads x page table too large (%.1e steps of %d keys, at most 4e9)", most, a.step);
   const long long slots = 2ll * ctas_of(a) * a.rows;
   a.part = static_cast<float*>(a.workspace);
   a.stat = reinterpret_cast<float2*>(a.part + slots * a.cache.D);
-  return slots * (a.cache.D * 4 + 8);
+  return a.cluster ? 0 : slots * (a.cache.D * 4 + 8);
 }
 
 }  // namespace
@@ -630,7 +728,7 @@ extern "C" int mpsa_kv_attention(const mpsa_kv_attention_args* args, void* strea
   if (!a.q || !a.out || !a.status) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: null pointer");
   if ((a.q_sb | a.q_sh | a.q_sl | a.o_sb | a.o_sh | a.o_sl) % 8 || ((uintptr_t)a.q | (uintptr_t)a.out) % 16)
     return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: q and out need 16-byte aligned bases and strides that are multiples of 8 elements");
-  if (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 256)
+  if (need && (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 256))
     return set_error(MPSA_ERR_BAD_ARG, "kv_attention: the workspace must hold %lld bytes and be 256-byte aligned", need);
   const cudaStream_t st = (cudaStream_t)stream;
   return a.dtype == 0 ? launch_all<__nv_bfloat16>(a, st) : launch_all<__half>(a, st);

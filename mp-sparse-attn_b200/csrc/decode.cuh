@@ -15,6 +15,7 @@ struct Call : mpsa_kv_attention_args {
   int step;                                    // keys of a step
   int least;                                   // steps of a run at least
   int groups;                                  // units of a (sequence, KV head)
+  int cluster;                                 // CTAs of a unit: nobody else has part of it, and there are no runs (0: runs)
   float* part;                                 // [2 x CTAs][rows][D], a CTA's run has at most two units that it shares with others
   float2* stat;                                // [2 x CTAs][rows]: row reference (log2), denominator relative to it
 };
