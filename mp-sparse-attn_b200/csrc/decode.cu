@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != 
   const int G = a.Hq / c.Hkv, R = a.T * G, units = c.Hkv * a.groups;
   const uint32_t mat = (lane & 15) * Y::row + ((lane >> 4) ^ Y::swap(lane & 15)) * 16;  // this lane's row address for ldmatrix
 
+  grid_dependency_wait();
   grid_dependents_go();
   uint32_t share, begin = 0, at = 0, stop = 1;
   int b = CLUSTER ? blockIdx.x / a.cluster / units : locate(a, gridDim.x, blockIdx.x, share, begin, lane);
@@ -639,19 +640,21 @@ int launch(const Call& a, int ctas, cudaStream_t st) {
       cfg.blockDim = dim3(32 * kWarps);
       cfg.dynamicSmemBytes = bytes;
       cfg.stream = st;
-      cudaLaunchAttribute at[1];
+      cudaLaunchAttribute at[2];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = a.cluster;
       at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[1].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = at;
-      cfg.numAttrs = 1;
+      cfg.numAttrs = overlaps_previous(st) ? 2 : 1;
       cudaLaunchKernelEx(&cfg, kernel, a);
       return check_launch("kv_attention");
     }
   }
   const auto kernel = kv_attention_kernel<T, ELEM, D, NR, false>;
   if (!allow_smem<id>(kernel, bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-  kernel<<<ctas, 32 * kWarps, bytes, st>>>(a);
+  launch_dependent(kernel, dim3(ctas), 32 * kWarps, bytes, st, overlaps_previous(st), a);
   return check_launch("kv_attention");
 }
 template <typename T, int ELEM, int D>

@@ -214,7 +214,6 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = a.Hq / a.cache.Hkv, R = a.T * G;
 
-  grid_dependents_go();
   if (warp == 7) {
     tmem_alloc(&sh.tmem, kColumns);
     if (lane == 0) {
@@ -233,6 +232,8 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  grid_dependency_wait();
+  grid_dependents_go();
 
   Run run(a, lane);
   uint32_t n = 0;                                      // steps so far: every barrier but q_full completes once a step
@@ -580,7 +581,7 @@ template <typename T, int ELEM, int D>
 int launch(const Call& a, int ctas, cudaStream_t st) {
   constexpr int id = 100000 + (std::is_same_v<T, __half> ? 1 : 0) + ELEM * 10 + D * 100;
   if (!allow_smem<id>(kv_attention_wide_kernel<T, ELEM, D>, Layout<D>::bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-  kv_attention_wide_kernel<T, ELEM, D><<<ctas, kThreads, Layout<D>::bytes, st>>>(a);
+  launch_dependent(kv_attention_wide_kernel<T, ELEM, D>, dim3(ctas), kThreads, Layout<D>::bytes, st, overlaps_previous(st), a);
   return check_launch("kv_attention");
 }
 template <typename T, int ELEM>

@@ -35,7 +35,7 @@ __device__ __forceinline__ int block_exponent(uint32_t amax) {
 }
 
 template <int ELEM>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8]) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8], bool fine) {       // zeros where not fine
   if constexpr (ELEM == E2M1) {
     uint32_t r = 0;
 #pragma unroll
@@ -44,7 +44,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8]) {
       asm("{\n.reg .b8 h;\ncvt.rn.satfinite.e2m1x2.f32 h, %2, %1;\ncvt.u32.u8 %0, h;\n}" : "=r"(two) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
       r |= two << (8 * i);
     }
-    *reinterpret_cast<uint32_t*>(p) = r;
+    *reinterpret_cast<uint32_t*>(p) = fine ? r : 0u;
   } else {
     uint32_t r[2] = {};
 #pragma unroll
@@ -54,8 +54,28 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[8]) {
       else asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(two) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
       r[i / 2] |= (uint32_t)two << (16 * (i % 2));
     }
-    *reinterpret_cast<uint2*>(p) = make_uint2(r[0], r[1]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(fine ? r[0] : 0u, fine ? r[1] : 0u);
   }
+}
+
+// The largest magnitude of 8 elements, as the bits of an fp32 number: a NaN is the largest.  16-bit elements two at a time.
+__device__ __forceinline__ uint32_t magnitude(const Raw4<__nv_bfloat16> (&r)[2]) {
+  const uint32_t m = 0x7fff7fffu;
+  const uint32_t a = __vmaxu2(__vmaxu2(r[0].u.x & m, r[0].u.y & m), __vmaxu2(r[1].u.x & m, r[1].u.y & m));
+  return max(a << 16, a & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t magnitude(const Raw4<__half> (&r)[2]) {
+  const uint32_t m = 0x7fff7fffu;
+  const uint32_t a = __vmaxu2(__vmaxu2(r[0].u.x & m, r[0].u.y & m), __vmaxu2(r[1].u.x & m, r[1].u.y & m));
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(a & 0xffffu, a >> 16))));
+}
+__device__ __forceinline__ uint32_t magnitude(const Raw4<float> (&r)[2]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    a = max(max(a, max(__float_as_uint(r[i].u.x) & 0x7fffffffu, __float_as_uint(r[i].u.y) & 0x7fffffffu)),
+            max(__float_as_uint(r[i].u.z) & 0x7fffffffu, __float_as_uint(r[i].u.w) & 0x7fffffffu));
+  return a;
 }
 
 // D/8 lanes take a row of K and the same row of V, 8 elements each; 4 lanes share a block of 32.  U tokens a group, all requested before the
@@ -66,9 +86,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const int j = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
   const int t0 = blockIdx.x * (kRows * U) + threadIdx.x / LANES;
   const mpsa_kv_cache& c = a.cache;
+  grid_dependency_wait();
+  grid_dependents_go();
   const T* const k = static_cast<const T*>(a.k) + b * a.k_sb + h * a.k_sh + 8 * j;
   const T* const v = static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh + 8 * j;
-  Raw4<T> raw[U][2][2];
+  Raw4<T> raw[U][2][2] = {};
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int t = t0 + i * kRows;
@@ -93,29 +115,19 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     const long long row = (((long long)max(page[i], 0) * c.Hkv + h) << shift) + ((start + t0 + i * kRows) & (c.page_size - 1));
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      float x[8];
-      if (page[i] >= 0) {
-        float lo[4], hi[4];
-        wide4(raw[i][o][0], lo);
-        wide4(raw[i][o][1], hi);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-      }
-      uint32_t amax = 0;                                          // as bits: a NaN is the largest
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+      uint32_t amax = page[i] >= 0 ? magnitude(raw[i][o]) : 0u;
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const bool fine = amax < 0x7f800000u;
       const int s = fine ? block_exponent<ELEM>(amax) : 128;
       const float r = __uint_as_float((uint32_t)(127 - s) << 23);  // exact: s is -126 .. 126
+      float lo[4], hi[4], x[8];
+      wide4(raw[i][o][0], lo);
+      wide4(raw[i][o][1], hi);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fine ? x[e] * r : 0.0f;
+      for (int e = 0; e < 4; ++e) x[e] = lo[e] * r, x[4 + e] = hi[e] * r;
       if (page[i] >= 0) {
-        store_codes<ELEM>(static_cast<uint8_t*>(o ? c.v : c.k) + row * code_bytes(ELEM, D) + code_bytes(ELEM, 8 * j), x);
+        store_codes<ELEM>(static_cast<uint8_t*>(o ? c.v : c.k) + row * code_bytes(ELEM, D) + code_bytes(ELEM, 8 * j), x, fine);
         if (j % 4 == 0) static_cast<uint8_t*>(o ? c.v_scale : c.k_scale)[row * NB + j / 4] = (uint8_t)(s + 127);
       }
     }
@@ -156,6 +168,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   const int j = threadIdx.x % LANES, h = blockIdx.y, b = blockIdx.z;
   const int t0 = blockIdx.x * (kRows * U) + threadIdx.x / LANES;
   const mpsa_kv_cache& c = a.cache;
+  grid_dependency_wait();
+  grid_dependents_go();
   const int n = min(a.lengths[b], a.max_len), shift = __popc(c.page_size - 1);
   Codes<ELEM> code[U][2];
   uint32_t scale[U][2];
@@ -192,17 +206,17 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   }
 }
 
-// Tokens of a lane group: 4 where there are enough for that.  (2 x 4099 tokens of 8 heads: 14.6 us with one, one 512-token chunk 4.6.)
-constexpr int kAppendRows = 4, kReadRows = 2;
+// Tokens of a lane group, where there are enough of them for eight CTAs an SM.  2 x 4099 tokens of 8 heads appended, calls back to back: 12.7 us
+// with two, 13.4 with four; prefixes of 4 x 8192 read 35.2 us with one, two or four.
+constexpr int kAppendRows = 2, kReadRows = 2;
 
 template <typename T, int ELEM, int LANES>
 void append_lanes(const mpsa_kv_append_args& a, cudaStream_t st) {
   constexpr int rows = kThreads / LANES;
-  const bool many = a.T > rows;
+  const bool many = (long long)a.T * a.cache.Hkv * a.B > 8ll * kAppendRows * rows * sm_count();
   const int per = many ? kAppendRows * rows : rows;
   const dim3 grid((a.T + per - 1) / per, a.cache.Hkv, a.B);
-  if (many) kv_append_kernel<T, ELEM, LANES, kAppendRows><<<grid, kThreads, 0, st>>>(a);
-  else kv_append_kernel<T, ELEM, LANES, 1><<<grid, kThreads, 0, st>>>(a);
+  launch_dependent(many ? kv_append_kernel<T, ELEM, LANES, kAppendRows> : kv_append_kernel<T, ELEM, LANES, 1>, grid, kThreads, 0, st, overlaps_previous(st), a);
 }
 template <typename T, int ELEM>
 int append_as(const mpsa_kv_append_args& a, cudaStream_t st) {
@@ -219,8 +233,7 @@ template <typename T, int ELEM>
 int read_as(const mpsa_kv_read_args& a, cudaStream_t st) {
   const int rows = kThreads / (a.cache.D / 8) * kReadRows;
   const dim3 grid((a.max_len + rows - 1) / rows, a.cache.Hkv, a.B);
-  if (a.cache.D == 64) kv_read_kernel<T, ELEM, 8, kReadRows><<<grid, kThreads, 0, st>>>(a);
-  else kv_read_kernel<T, ELEM, 16, kReadRows><<<grid, kThreads, 0, st>>>(a);
+  launch_dependent(a.cache.D == 64 ? kv_read_kernel<T, ELEM, 8, kReadRows> : kv_read_kernel<T, ELEM, 16, kReadRows>, grid, kThreads, 0, st, overlaps_previous(st), a);
   return check_launch("kv_read");
 }
 template <typename T>

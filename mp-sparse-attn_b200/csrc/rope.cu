@@ -114,6 +114,8 @@ __global__ void __launch_bounds__(kThreads, 4) norm_rope_heads_kernel(const __gr
   const bool live = n < (long long)a.B * a.L;
   const int b = live ? (int)(n / a.L) : 0, l = live ? (int)(n % a.L) : 0;
   const Place p = place(j, a.cos ? a.rot : 0, INTERLEAVED);
+  grid_dependency_wait();
+  grid_dependents_go();
   float c[4] = {1, 1, 1, 1}, s[4] = {};
   if (p.turned) angles(a, b, l, j, c, s);
 #pragma unroll
@@ -176,6 +178,8 @@ __global__ void __launch_bounds__(256, 3) norm_rope_across_kernel(const __grid_c
   const T* x = static_cast<const T*>(a.x[o]) + (b * a.x_sb[o] + l * a.x_sl[o] + group * a.x_sh[o]);
   T* y = static_cast<T*>(a.y[o]) + (b * a.y_sb[o] + l * a.y_sl[o] + group * a.y_sh[o]);
   const long long xh = groups * a.x_sh[o], yh = groups * a.y_sh[o];
+  grid_dependency_wait();
+  grid_dependents_go();
   Raw4<T> r0[kChunks], r1[kChunks];
 #pragma unroll
   for (int k = 0; k < kChunks; ++k) {
@@ -248,14 +252,14 @@ int launch(NormRope& a, cudaStream_t st) {
   if (a.norm == 2) {
     const int most = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
     const int threads = (most * LANES + 32 * kChunks - 1) / (32 * kChunks) * 32;
-    norm_rope_across_kernel<T, W, LANES, INTERLEAVED><<<dim3((unsigned)tokens, a.x[1] ? 2 : 1), threads, 0, st>>>(a);
+    launch_dependent(norm_rope_across_kernel<T, W, LANES, INTERLEAVED>, dim3((unsigned)tokens, a.x[1] ? 2 : 1), threads, 0, st, overlaps_previous(st), a);
     return check_launch("norm_rope");
   }
   const long long groups = (tokens + kThreads / LANES - 1) / (kThreads / LANES);
   a.heads_per_cta = heads;                                           // split over CTAs where there are few tokens
   while (a.heads_per_cta > kAhead && groups * ((heads + a.heads_per_cta - 1) / a.heads_per_cta) < 8ll * sm_count()) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid((unsigned)groups, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
-  norm_rope_heads_kernel<T, W, LANES, INTERLEAVED><<<grid, kThreads, 0, st>>>(a);
+  launch_dependent(norm_rope_heads_kernel<T, W, LANES, INTERLEAVED>, grid, kThreads, 0, st, overlaps_previous(st), a);
   return check_launch("norm_rope");
 }
 template <typename T, typename W>
