@@ -27,7 +27,7 @@ namespace mpsa {
 namespace {
 
 constexpr int kWarps = 4, kStep = 32;
-constexpr int kMostCluster = 8, kClusterSteps = 64;
+constexpr int kMostCluster = 8, kClusterSteps = 40;
 constexpr float kMost = 15.0f, kSet = 7.0f;    // log2 of the largest product that raises no reference, and of the largest one after a raise
 constexpr int kLeast = -85;                    // log2 of a scale that counts as that at least: references are the largest score - 100 at least
 
@@ -110,6 +110,10 @@ __device__ __forceinline__ void v_fragments(uint32_t p, uint32_t (&f)[ELEM == E2
     }
 }
 
+// CTAs of an SM: what shared memory (four-bit codes need half) and registers let in.  16 rows of depth 128 spill with three: 8 sequences of 8192
+// with 4 x 4 rows 60.8 us, with two 41.7.
+constexpr __host__ __device__ int per_sm(int tiles, int elem, int D) { return tiles == 4 || (tiles == 2 && D == 128) ? 2 : tiles == 2 || elem != E2M1 ? 3 : 4; }
+
 // Cluster barrier: what its CTAs wrote to shared memory before it can be read by all of them after it.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -143,7 +147,7 @@ __device__ __forceinline__ void write_out(const Call& a, int b, int h, int G, in
 
 // CLUSTER: a.cluster CTAs share a unit, each has an equal run of its steps, and they add up their parts through shared memory.
 template <typename T, int ELEM, int D, int NR, bool CLUSTER>
-__global__ void __launch_bounds__(32 * kWarps, NR == 4 ? 2 : NR == 2 || ELEM != E2M1 ? 3 : 4) kv_attention_kernel(const __grid_constant__ Call a) {
+__global__ void __launch_bounds__(32 * kWarps, per_sm(NR, ELEM, D)) kv_attention_kernel(const __grid_constant__ Call a) {
   using Y = Layout<ELEM, D, NR>;
   constexpr int NB = D / 32, NM = kStep / 16;          // blocks of the depth, key tiles of a step
   constexpr int BP = ELEM == E2M1 ? 2 : 1;             // blocks of a 32-byte piece
@@ -621,9 +625,9 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
 
 bool wide(const Call& a) { return a.rows == kWideRows; }
 
-int ctas_of(const Call& a) {                          // of an SM: as many as registers and shared memory let in
+int ctas_of(const Call& a) {
   const double most = (double)a.B * a.cache.Hkv * a.groups * ((double)a.max_pages * a.cache.page_size / a.step + 1);
-  const double all = (double)(wide(a) ? kWideCtas : a.rows == 32 ? 2 : a.rows == 16 || a.cache.elem != E2M1 ? 3 : 4) * sm_count();
+  const double all = (double)(wide(a) ? kWideCtas : per_sm(a.rows / 8, a.cache.elem, a.cache.D)) * sm_count();
   return (int)(most < all ? most : all);
 }
 
@@ -679,8 +683,10 @@ int launch_all(const Call& a, cudaStream_t st) {
   return check_launch("kv_attention");
 }
 
-// CTAs of a cluster for each unit, or 0 for runs and the combining launch.  Clusters where the table holds so little that a unit's steps keep
-// few warps busy for a short time: then the combining launch costs more than what equal runs gain with uneven lengths.
+// CTAs of a cluster for each unit, or 0 for runs and the combining launch.  Clusters where the table holds so little that the combining launch
+// costs more than what equal runs gain.  8 KV heads of depth 128 in E4M3, tables as long as the sequences, us with clusters / with runs: one
+// sequence of 2048 7.6 / 9.6, 8192 13.9 / 19.0, 16384 22.2 / 21.2; 8 of 4096 20.3 / 20.7 (uneven lengths 14.8 / 16.5); 32 of 1024 19.6 / 20.5
+// (14.5 / 17.8), 32 of 2048 35.2 / 32.0 (24.6 / 20.8).
 int cluster_of(const Call& a) {
   if (a.rows > 16) return 0;
   const double units = (double)a.B * a.cache.Hkv * a.groups, room = 3.0 * sm_count(), steps = (double)a.max_pages * a.cache.page_size / a.step;
@@ -701,12 +707,14 @@ long long plan(const mpsa_kv_attention_args* args, Call& a) {
   if (a.B > 65535 || a.Hq > 65535 || a.T > 1024) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: at most 65535 sequences and 1024 query tokens");
   if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f) return set_error(MPSA_ERR_BAD_ARG, "kv_attention: sm_scale must be positive and finite");
   const int rows = a.T * (a.Hq / a.cache.Hkv);
+  // (8 sequences of 8192, 4 query heads a KV head, 128 keys a step / 32 keys, us: 32 rows 70.7 / 64.7, 40 rows 74.3 / 109.8, 96 rows 83.6 / 155.7)
   a.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : kWideRows;
   a.step = wide(a) ? kWideStep : kStep;
   a.least = wide(a) ? 2 : 4;                          // (four: a step for each warp)
   a.groups = (rows + a.rows - 1) / a.rows;
   a.cluster = cluster_of(a);
   const double most = (double)a.B * a.cache.Hkv * a.groups * ((double)a.max_pages * a.cache.page_size / a.step + 1);
+  if ((double)a.B * a.cache.Hkv * a.groups > 2147483647.0) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: too many sequences and heads");
   if (most > 4e9) return set_error(MPSA_ERR_UNSUPPORTED, "kv_attention: sequences x heads x page table too large (%.1e steps of %d keys, at most 4e9)", most, a.step);
   const long long slots = 2ll * ctas_of(a) * a.rows;
   a.part = static_cast<float*>(a.workspace);

@@ -21,7 +21,7 @@ struct Call : mpsa_kv_attention_args {
 };
 
 __device__ __forceinline__ int length_of(const Call& a, int b) {
-  return min(max(a.lengths[b], 0), (int)min(0x7fffffc0ll, (long long)a.max_pages * a.cache.page_size));
+  return min(max(a.lengths[b], 0), (int)min(0x7ffffe00ll, (long long)a.max_pages * a.cache.page_size));
 }
 __device__ __forceinline__ int queries_of(const Call& a, int b, int len) { return min(a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T, len); }
 __device__ __forceinline__ int steps_of(const Call& a, int len) { return max(1, (len + a.step - 1) / a.step); }    // (an empty sequence: one, which writes its zeros)

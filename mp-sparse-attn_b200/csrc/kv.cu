@@ -15,6 +15,7 @@ int check_cache(const mpsa_kv_cache& c, const char* what) {
   if (c.num_pages <= 0 || c.Hkv <= 0 || c.Hkv > 65535) return set_error(MPSA_ERR_BAD_ARG, "%s: the cache needs pages and 1 to 65535 heads", what);
   if (c.page_size < 16 || c.page_size > 1024 || (c.page_size & (c.page_size - 1)))
     return set_error(MPSA_ERR_UNSUPPORTED, "%s: page_size must be a power of two from 16 to 1024", what);
+  if ((double)c.num_pages * c.Hkv * c.page_size >= 4294967295.0) return set_error(MPSA_ERR_UNSUPPORTED, "%s: the cache may have 2^32 - 2 rows at most", what);
   return MPSA_OK;
 }
 

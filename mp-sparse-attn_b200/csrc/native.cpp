@@ -277,6 +277,8 @@ bool rows_aligned(const at::Tensor& t, int elements) {
          fits_int(t.size(2)) && fits_int(t.size(3));
 }
 
+bool asks_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
 // int32 [B], dense, on `device`
 bool indices(const at::Tensor& t, int64_t B, int device) {
   return t.dim() == 1 && t.size(0) == B && t.scalar_type() == at::kInt && t.is_contiguous() && t.get_device() == device;
@@ -326,10 +328,9 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int hnd = PyObject_IsTrue(a[11]), h = hnd ? 1 : 2, l = hnd ? 2 : 1;
     if (PyErr_Occurred()) return nullptr;
     if (c.in_dtype < 0 || (!c.norm && (w[0] || w[1])) || (!x[1] && w[1])) Py_RETURN_NONE;
-    const bool grad = at::GradMode::is_enabled();
     const int device = x[0]->get_device();
     for (int i = 0; i < (x[1] ? 2 : 1); ++i) {
-      if (!rows_aligned(*x[i], 4) || x[i]->scalar_type() != x[0]->scalar_type() || x[i]->get_device() != device || (grad && x[i]->requires_grad())) Py_RETURN_NONE;
+      if (!rows_aligned(*x[i], 4) || x[i]->scalar_type() != x[0]->scalar_type() || x[i]->get_device() != device || asks_gradient(*x[i])) Py_RETURN_NONE;
       const auto z = x[i]->sizes(), s = x[i]->strides();
       if (z[0] != x[0]->size(0) || z[l] != x[0]->size(l) || z[3] != x[0]->size(3)) Py_RETURN_NONE;
       c.x[i] = x[i]->data_ptr();
@@ -339,7 +340,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const int64_t D = z[3], most = c.norm == 2 ? z[h] * D : D;
       const bool shaped = w[i]->dim() == 1 ? w[i]->size(0) == most : w[i]->dim() == 2 && c.norm == 2 && w[i]->size(0) == z[h] && w[i]->size(1) == D;
       c.w_dtype[i] = any_dtype(*w[i]);
-      if (!shaped || (c.w_dtype[i] != 2 && c.w_dtype[i] != c.in_dtype) || (i && w[0] && c.w_dtype[0] != c.w_dtype[1]) || reinterpret_cast<uintptr_t>(w[i]->data_ptr()) % 16 || !w[i]->is_contiguous() || w[i]->get_device() != device || (grad && w[i]->requires_grad())) Py_RETURN_NONE;
+      if (!shaped || (c.w_dtype[i] != 2 && c.w_dtype[i] != c.in_dtype) || (i && w[0] && c.w_dtype[0] != c.w_dtype[1]) || reinterpret_cast<uintptr_t>(w[i]->data_ptr()) % 16 || !w[i]->is_contiguous() || w[i]->get_device() != device || asks_gradient(*w[i])) Py_RETURN_NONE;
       c.weight[i] = w[i]->data_ptr();
     }
     c.B = (int)x[0]->size(0); c.L = (int)x[0]->size(l); c.D = (int)x[0]->size(3);
@@ -405,7 +406,7 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *own = plain(a[1]), *k = plain(a[2]), *v = plain(a[3]), *table = plain(a[4]), *start = plain(a[5]), *counts;
     if (!cache || !own || !k || !v || !table || !start || !optional_plain(a[6], counts)) Py_RETURN_NONE;
     const int hnd = PyObject_IsTrue(a[7]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
-    if (!rows_aligned(*k, 8) || !rows_aligned(*v, 8) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || any_dtype(*k) < 0 ||
+    if (!rows_aligned(*k, 8) || !rows_aligned(*v, 8) || asks_gradient(*k) || asks_gradient(*v) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || any_dtype(*k) < 0 ||
         k->get_device() != device || v->get_device() != device || k->size(h) != cache->Hkv || k->size(3) != cache->D)
       Py_RETURN_NONE;
     const int64_t B = k->size(0);
@@ -475,7 +476,7 @@ PyObject* kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int lse = PyObject_IsTrue(a[9]), hnd = PyObject_IsTrue(a[10]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
     if (PyErr_Occurred()) return nullptr;
     c.dtype = in_dtype(*q);
-    if (c.dtype < 0 || !rows_aligned(*q, 8) || q->get_device() != device || q->size(3) != cache->D || q->size(h) % cache->Hkv || q->size(l) > 1024) Py_RETURN_NONE;
+    if (c.dtype < 0 || !rows_aligned(*q, 8) || asks_gradient(*q) || q->get_device() != device || q->size(3) != cache->D || q->size(h) % cache->Hkv || q->size(l) > 1024) Py_RETURN_NONE;
     const int64_t B = q->size(0), T = q->size(l), Hq = q->size(h);
     if (!page_table(*table, B, device) || !indices(*lengths, B, device) || (qlens && !indices(*qlens, B, device))) Py_RETURN_NONE;
     if (mask) {

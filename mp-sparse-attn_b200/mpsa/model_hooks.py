@@ -76,7 +76,37 @@ def add_mxfp_kernel(attention_class) -> None:
     attention_class.kernel_selection = kernel_selection
 
 
-def _wan_self_attention_forward(rope_apply: Callable):
+def grid_positions(grid, length: int, device=None) -> torch.Tensor:
+    """int32 [length, 3]: frame, row and column of the tokens of a (frames, height, width) grid in memory order.  Tokens behind the grid
+    (padding) have position 0 on every axis, where a rotary table does nothing."""
+    f, h, w = (int(n) for n in grid)
+    if f * h * w > length:
+        raise ValueError("the grid has more tokens than the sequence")
+    i = torch.arange(f * h * w, device=device)
+    pos = torch.zeros(length, 3, dtype=torch.int32, device=device)
+    pos[:f * h * w] = torch.stack((i // (h * w), i // w % h, i % w), 1).to(torch.int32)
+    return pos
+
+
+def _wan_norm_rope(attn, q, k, grid_sizes, freqs):
+    """norm_q, norm_k (RMS over all heads of a token) and rope_apply (pairs of neighbours; the table's columns split among frame, height and
+    width) of a Wan self-attention block in one pass; q, k [B,L,H,D]."""
+    from .serving import norm_rope
+    L, d = q.shape[1], q.shape[3]
+    half = d // 2
+    side = half // 3
+    weights = [getattr(n, "weight", None) for n in (attn.norm_q, attn.norm_k)]
+    if any(w is None for w in weights) and not all(isinstance(n, torch.nn.Identity) for n in (attn.norm_q, attn.norm_k)):
+        raise ValueError("fused_norm_rope needs RMS norms with weights, or none")
+    normed = weights[0] is not None
+    positions = torch.stack([grid_positions(g, L, q.device) for g in grid_sizes.tolist()])
+    freqs = freqs.to(q.device)
+    return norm_rope(q, k, q_weight=weights[0], k_weight=weights[1], norm=normed, across_heads=normed, eps=float(getattr(attn.norm_q, "eps", 1e-6)),
+                     rope=(freqs.real.float().contiguous(), freqs.imag.float().contiguous()), positions=positions,
+                     sections=(half - 2 * side, side, side), interleaved=True, tensor_layout="NHD")
+
+
+def _wan_self_attention_forward(rope_apply: Callable, fused: bool = False):
     @torch.no_grad()
     def forward(self, x, seq_lens, grid_sizes, freqs):
         """x [B, L, C]; seq_lens [B]; grid_sizes [B, 3]; freqs: rotary table (evaluate/modify_model/modify_wan.py:98-125)."""
@@ -85,10 +115,13 @@ def _wan_self_attention_forward(rope_apply: Callable):
             raise ValueError("windowed attention is not supported")
         if seq_lens.shape[0] != 1:
             raise ValueError("one sequence per call (no variable-length batches)")
-        q = self.norm_q(self.q(x)).view(b, s, n, d)
-        k = self.norm_k(self.k(x)).view(b, s, n, d)
         v = self.v(x).view(b, s, n, d)
-        q, k = rope_apply(q, grid_sizes, freqs), rope_apply(k, grid_sizes, freqs)
+        if fused:
+            q, k = _wan_norm_rope(self, self.q(x).view(b, s, n, d), self.k(x).view(b, s, n, d), grid_sizes, freqs)
+        else:
+            q = self.norm_q(self.q(x)).view(b, s, n, d)
+            k = self.norm_k(self.k(x)).view(b, s, n, d)
+            q, k = rope_apply(q, grid_sizes, freqs), rope_apply(k, grid_sizes, freqs)
         half = (torch.float16, torch.bfloat16)
         q, k, v = (t if t.dtype in half else t.to(torch.bfloat16) for t in (q, k, v))
         o = self.inner_attention(q, k.to(q.dtype), v.to(q.dtype), is_causal=False, tensor_layout="NHD")
@@ -97,14 +130,16 @@ def _wan_self_attention_forward(rope_apply: Callable):
 
 
 def set_mpsa_attn_wan(model, rope_apply: Optional[Callable] = None, block_scale_type: str = "diag_requant",
-                      smooth_k: bool = True) -> int:
+                      smooth_k: bool = True, fused_norm_rope: bool = False) -> int:
     """Every block's self-attention of a Wan model (`model.blocks[i].self_attn` with q/k/v/o projections, norm_q/norm_k,
     num_heads, head_dim) computes its attention with this library from now on; returns the number of blocks patched.
-    rope_apply: the model family's rotary function (default: wan.modules.model.rope_apply)."""
-    if rope_apply is None:
+    rope_apply: the model family's rotary function (default: wan.modules.model.rope_apply).
+    fused_norm_rope: norm_q, norm_k and the rotation of one block in one launch of this library's norm_rope, rounded once at the end
+    (rope_apply is then not called and not needed)."""
+    if rope_apply is None and not fused_norm_rope:
         from wan.modules.model import rope_apply as _rope_apply      # the model's own package
         rope_apply = _rope_apply
-    fwd = _wan_self_attention_forward(rope_apply)
+    fwd = _wan_self_attention_forward(rope_apply, fused_norm_rope)
     n = 0
     for block in model.blocks:
         block.self_attn.inner_attention = MixedPrecisionAttention(block_scale_type=block_scale_type, smooth_k=smooth_k)

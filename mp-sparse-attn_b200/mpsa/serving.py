@@ -7,7 +7,7 @@ tokens, chunks or trees of drafted tokens over it.  The reference has none of th
     mpsa.kv_cache_append(cache, k, v, page_table, lengths)              # tokens lengths[b] .. lengths[b] + T - 1
     o = mpsa.kv_cache_attention(q, cache, page_table, lengths + T)      # the last T tokens of each sequence
 
-No gradients: these are inference operations, and norm_rope refuses operands that ask for one.
+No gradients: these are inference operations, and operands that ask for one are refused.
 """
 from __future__ import annotations
 
@@ -62,6 +62,11 @@ def _aligned(x: torch.Tensor, tensor_layout: str, elements: int):
     return x, size, st
 
 
+def _no_gradient(*ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError("no gradient is computed here: call it under torch.no_grad()")
+
+
 def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Optional[torch.Tensor] = None,
               k_weight: Optional[torch.Tensor] = None, norm: bool = True, across_heads: bool = False, eps: float = 1e-6, rope=None,
               positions: Optional[torch.Tensor] = None, sections: Optional[Tuple[int, ...]] = None, interleaved: bool = False,
@@ -85,8 +90,7 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
             _lib.check(r)
         return r
     _require_cuda(q, k, q_weight, k_weight, positions)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        raise ValueError("norm_rope computes no gradient: call it under torch.no_grad()")
+    _no_gradient(q, k, q_weight, k_weight)
     if q.dtype not in _IN_DTYPE:
         raise ValueError(f"unsupported input dtype {q.dtype}")
     a = _NormRopeArgs()
@@ -163,7 +167,7 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
     return tuple(outs) if k is not None else outs[0]
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KVCache:
     """A paged cache of keys and values in MX blocks of 32 along the depth, quantised token by token: what kv_cache() makes, or a program's own buffers.
 
@@ -179,8 +183,9 @@ class KVCache:
     def __post_init__(self):
         if self.elem not in _ELEM:
             raise ValueError(f"unknown cache element {self.elem!r}")
-        self._c = _lib.native().kv_cache(self.k, self.k_scale, self.v, self.v_scale, _ELEM[self.elem])       # the argument block, as bytes
-        if self._c is not None:
+        block = _lib.native().kv_cache(self.k, self.k_scale, self.v, self.v_scale, _ELEM[self.elem])         # the argument block, as bytes
+        if block is not None:
+            object.__setattr__(self, "_c", block)
             return
         _require_cuda(self.k, self.v, self.k_scale, self.v_scale)
         if self.k.dim() != 4:
@@ -190,8 +195,8 @@ class KVCache:
         for t, n in ((self.k, row), (self.v, row), (self.k_scale, D // 32), (self.v_scale, D // 32)):
             if t.dtype is not torch.uint8 or t.shape != (pages, heads, page, n) or not t.is_contiguous() or t.device != self.k.device:
                 raise ValueError("cache buffers must be contiguous uint8 [pages, heads, page size, ...] on one device")
-        self._c = bytes(_Cache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), pages, page, heads, D,
-                               _ELEM[self.elem]))
+        object.__setattr__(self, "_c", bytes(_Cache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), pages,
+                                                    page, heads, D, _ELEM[self.elem])))
 
     @property
     def num_kv_heads(self) -> int:
@@ -249,6 +254,7 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
         if r is not None:
             return _lib.check(r)
     _require_cuda(k, v, page_table, start, counts)
+    _no_gradient(k, v)
     if k.dtype not in _IN_DTYPE or v.dtype != k.dtype:
         raise ValueError(f"unsupported input dtypes {k.dtype}, {v.dtype}")
     dev = cache.k.device
@@ -301,7 +307,7 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
 
     q [B,Hq,T,D] (or NHD), bf16 or fp16, T up to 1024; Hq a multiple of the cache's heads; the result has q's shape and type.
     lengths int32 [B]: tokens in the cache, the query tokens among them (append them first).  q_lens int32 [B]: how many of the T are real
-    (the first ones; the rows behind them come back as zero); None: all.
+    (the first ones; the rows behind them come back as zero); None: all, or lengths[b] where that is fewer.
     mask: bool [T,T] or [B,T,T], True where query token i sees query token j - a tree of drafted tokens; None: every token sees those before
     it and itself.  Cached tokens before the query tokens are seen by all.  A row that sees nothing is zero.
     return_lse: also fp32 [B,Hq,T], log2 of the softmax denominators (-inf for a row that sees nothing), as attention_merge takes it."""
@@ -317,6 +323,7 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
                 _lib.check(r)
             return r
     _require_cuda(q, page_table, lengths, q_lens, mask)
+    _no_gradient(q)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"unsupported query dtype {q.dtype}")
     if q.device != dev:

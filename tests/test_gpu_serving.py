@@ -1,4 +1,5 @@
 """Norm and rotation, the paged MX cache and attention over it, against plain 64-bit forms (serving_plain.py)."""
+import importlib.util
 import math
 import os
 import sys
@@ -595,6 +596,182 @@ def test_parts_merge():
     acc, l = parts[0][0].float(), parts[0][1].clone()
     mpsa.attention_merge(acc, l, parts[1][0], parts[1][1])
     assert float((acc - whole.float()).abs().max()) <= 2 * half_step(BF16) * float(whole.abs().max()) and float((l - lse).abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("elem,D", [("e4m3", 128), ("e2m1", 64), ("e5m2", 64), ("e2m1", 128)])
+@pytest.mark.parametrize("T,Hq", [(1, 8), (3, 8), (7, 8), (40, 8)])
+def test_attention_whose_units_are_cut_anywhere(elem, D, T, Hq):
+    """Tables that are long enough for runs of equal length: units begin and end in the middle of them, some CTAs have several, some none."""
+    import mpsa
+    g = torch.Generator().manual_seed(T + D)
+    lens = [3000, T, 800, 0, 61, 4100, 33]
+    q_lens = [T, T, max(1, T - 2), 0, T, T, 1]
+    lens = [max(n, t) for n, t in zip(lens, q_lens)]
+    c, table = real_cache(g, 7, lens, 2, 64, D, elem, amp=0.7)
+    table = torch.cat((table, torch.full((7, 256), -1, dtype=torch.int32)), 1)            # room for more than they have
+    q = rnd(g, 7, Hq, T, D)
+    args = (q.cuda(), c, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    kw = dict(q_lens=torch.tensor(q_lens, dtype=torch.int32).cuda(), return_lse=True)
+    out, lse = mpsa.kv_cache_attention(*args, **kw)
+    check_attention(c, table, lens, q, out.cpu(), lse.cpu(), q_lens)
+    again = mpsa.kv_cache_attention(*args, **kw)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    mpsa.check_status()
+
+
+def test_many_sequences():
+    import mpsa
+    g = torch.Generator().manual_seed(20)
+    B = 300
+    lens = [int(x) for x in torch.randint(0, 90, (B,), generator=g)]
+    lens[7], lens[250] = 1500, 700
+    c, table = real_cache(g, B, lens, 1, 16, 64, "e4m3")
+    for T, Hq in ((1, 2), (2, 20)):
+        q = rnd(g, B, Hq, T, 64)
+        q_lens = [min(T, n) for n in lens]
+        out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), return_lse=True)
+        check_attention(c, table, lens, q, out.cpu(), lse.cpu(), q_lens)
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_attention_captured_beside_another_stream(T):
+    """Graphs of two calls replayed at once on two streams, with new lengths, and an eager call between them."""
+    import mpsa
+    g = torch.Generator().manual_seed(21)
+    lens = [3000, 40, 7000]
+    c, table = real_cache(g, 3, [7100] * 3, 2, 64, 128, "e4m3")
+    table = table.cuda()
+    qs = [rnd(g, 3, 8, T, 128).cuda() for _ in range(2)]
+    lengths = [torch.tensor(lens, dtype=torch.int32).cuda() for _ in range(2)]
+    mpsa.kv_cache_attention(qs[0], c, table, lengths[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q, n in zip(qs, lengths):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(mpsa.kv_cache_attention(q, c, table, n))
+        graphs.append(graph)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(4):
+        lengths[0].add_(i)
+        lengths[1].copy_(torch.tensor([T + i, 7000 - 3 * i, 900], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for s, graph in zip(side, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = [mpsa.kv_cache_attention(q, c, table, n) for q, n in zip(qs, lengths)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+    mpsa.check_status()
+
+
+def test_long_chains_of_calls_see_what_was_written_before():
+    """Append, read and attention one behind the other without a host wait: each overlaps the launch of the one before."""
+    import mpsa
+    g = torch.Generator().manual_seed(22)
+    c = mpsa.kv_cache(64, 2, 128, page_size=16)
+    table = table_of(g, 2, 32, 64).cuda()
+    lengths = torch.zeros(2, dtype=torch.int32).cuda()
+    ks, vs = rnd(g, 2, 2, 60, 128).cuda(), rnd(g, 2, 2, 60, 128).cuda()
+    got = []
+    for t in range(60):
+        mpsa.kv_cache_append(c, ks[:, :, t:t + 1], vs[:, :, t:t + 1], table, lengths)
+        lengths += 1
+        got.append((mpsa.kv_cache_read(c, table, lengths, max_len=60), mpsa.kv_cache_attention(ks[:, :, t:t + 1], c, table, lengths)))
+    k, v = mpsa.kv_cache_read(c, table, lengths, max_len=60)
+    for t, ((a, b), o) in enumerate(got):
+        assert torch.equal(a[:, :, :t + 1], k[:, :, :t + 1]) and torch.equal(b[:, :, :t + 1], v[:, :, :t + 1]) and bool((a[:, :, t + 1:] == 0).all())
+        again = mpsa.kv_cache_attention(ks[:, :, t:t + 1], c, table, torch.full((2,), t + 1, dtype=torch.int32).cuda())
+        assert torch.equal(o, again)
+
+
+def test_the_long_way_gives_the_same(monkeypatch):
+    """Without the native module every call goes through the Python checks and ctypes."""
+    import mpsa
+    from mpsa import _lib
+    g = torch.Generator().manual_seed(23)
+    q, k, v = rnd(g, 2, 8, 5, 128).cuda(), rnd(g, 2, 2, 5, 128).cuda(), rnd(g, 2, 2, 5, 128).cuda()
+    cos, sin = (t.cuda() for t in _angles(64, 64))
+    lengths = torch.tensor([7, 30], dtype=torch.int32).cuda()
+    mask = tree_mask(g, 5).cuda()
+
+    def everything():
+        c = mpsa.kv_cache(8, 2, 128, page_size=16, elem="e5m2")
+        table = torch.arange(8, dtype=torch.int32).reshape(2, 4).cuda()
+        y = mpsa.norm_rope(q, k, q_weight=cos[0].repeat(2).contiguous(), rope=(cos, sin), positions=lengths[:, None] + torch.arange(5, dtype=torch.int32).cuda())
+        mpsa.kv_cache_append(c, y[1], v, table, lengths, counts=torch.tensor([5, 4], dtype=torch.int32).cuda())
+        r = mpsa.kv_cache_read(c, table, lengths + 5)
+        return (*y, c.k, c.v_scale, *r, *mpsa.kv_cache_attention(y[0], c, table, lengths + 5, mask=mask, return_lse=True), mpsa.norm_rope(q))
+
+    native = everything()
+    monkeypatch.setattr(_lib, "_native", _lib._LongWay)
+    assert all(torch.equal(a, b) for a, b in zip(native, everything()))
+
+
+def test_a_cache_keeps_its_buffers():
+    import dataclasses
+
+    import mpsa
+    c = mpsa.kv_cache(4, 1, 64)
+    with pytest.raises(dataclasses.FrozenInstanceError):
+        c.k = torch.zeros_like(c.k)
+    assert (c.num_kv_heads, c.page_size, c.head_dim) == (1, 64, 64) and mpsa.kv_cache(4, 3, 128, page_size=16, elem="e2m1").head_dim == 128
+    x = torch.zeros(1, 1, 2, 64, device="cuda", dtype=BF16, requires_grad=True)
+    i = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for f in (lambda: mpsa.kv_cache_append(c, x, x, i[None], i), lambda: mpsa.kv_cache_attention(x, c, i[None], i + 2)):
+        with pytest.raises(ValueError):
+            f()
+        with torch.no_grad():
+            f()
+
+
+# ------------------------------------------------------------------------------------------------------------------ model hook
+class _Rms(torch.nn.Module):
+    def __init__(self, dim):
+        super().__init__()
+        self.eps, self.weight = 1e-5, torch.nn.Parameter(1 + 0.2 * torch.randn(dim))
+
+    def forward(self, x):
+        return (x.double() * torch.rsqrt(x.double().pow(2).mean(-1, keepdim=True) + self.eps) * self.weight.double()).to(x.dtype)
+
+
+@pytest.mark.parametrize("normed", [True, False])
+def test_wan_block_with_norm_and_rotation_in_one_pass(normed):
+    from mpsa import model_hooks as H
+    spec = importlib.util.spec_from_file_location("_hooks_cpu", os.path.join(os.path.dirname(__file__), "test_model_hooks_cpu.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    torch.manual_seed(3)
+    heads, d, L, grid = 3, 128, 200, (4, 6, 8)
+    model = mod._Wan(dim=heads * d, heads=heads, n=1)
+    att = model.blocks[0].self_attn
+    if normed:
+        att.norm_q, att.norm_k = _Rms(heads * d), _Rms(heads * d)
+    model = model.cuda()
+    ang = torch.arange(64, dtype=torch.float64)[:, None] * torch.cat([1e4 ** (-torch.arange(n, dtype=torch.float64) / n) for n in (22, 21, 21)])
+    freqs = torch.polar(torch.ones_like(ang), ang)
+    H.set_mpsa_attn_wan(model, fused_norm_rope=True)
+    seen = []
+
+    class Recorder(torch.nn.Module):
+        def forward(self, q, k, v, **kw):
+            seen.append((q, k, kw))
+            return v
+
+    att.inner_attention = Recorder()
+    x = torch.randn(1, L, heads * d, device="cuda")
+    att(x, torch.tensor([L]), torch.tensor([grid]), freqs)
+    (q, k, kw), = seen
+    assert kw == dict(is_causal=False, tensor_layout="NHD") and q.dtype == BF16
+    f, h, w = grid
+    i = torch.arange(f * h * w)
+    turn = torch.cat((freqs[i // (h * w), :22], freqs[i // w % h, 22:43], freqs[i % w, 43:]), 1)[None, :, None]
+    for got, lin, norm in ((q, att.q, att.norm_q), (k, att.k, att.norm_k)):
+        y = norm(lin(x).detach()).double().cpu().reshape(1, L, heads, d)
+        z = torch.view_as_complex(y[:, :f * h * w].reshape(1, -1, heads, 64, 2).contiguous()) * turn
+        y[:, :f * h * w] = torch.view_as_real(z).flatten(-2)
+        # fp32 throughout (2^-24 of a few operations of elements of size 6 at most; the norm above rounds to fp32 once more), then bf16
+        assert bool(((got.double().cpu() - y).abs() <= half_step(BF16) * y.abs() * 1.01 + 2.0 ** -17).all())
 
 
 # ------------------------------------------------------------------------------------------------------------------ refusals

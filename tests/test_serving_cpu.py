@@ -174,3 +174,12 @@ def test_the_plain_rounding_is_the_nearest_value(elem):
     assert bool((b.abs().amax(-1) <= P.LARGEST[elem]).all()) and bool((b.abs().amax(-1) > P.LARGEST[elem] / 2).all())
     best = (b.unsqueeze(-1) - t).abs().amin(-1)
     assert torch.equal((b - y).abs(), best)
+
+
+def test_grid_positions():
+    from mpsa.model_hooks import grid_positions
+    p = grid_positions((2, 3, 4), 30)
+    assert p.shape == (30, 3) and p.dtype == torch.int32
+    assert p[:24].tolist() == [[f, h, w] for f in range(2) for h in range(3) for w in range(4)] and int(p[24:].abs().sum()) == 0
+    with pytest.raises(ValueError):
+        grid_positions((2, 3, 4), 23)
