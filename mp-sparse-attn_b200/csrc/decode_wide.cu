@@ -580,8 +580,9 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
 template <typename T, int ELEM, int D>
 int launch(const Call& a, int ctas, cudaStream_t st) {
   constexpr int id = 100000 + (std::is_same_v<T, __half> ? 1 : 0) + ELEM * 10 + D * 100;
-  if (!allow_smem<id>(kv_attention_wide_kernel<T, ELEM, D>, Layout<D>::bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
-  launch_dependent(kv_attention_wide_kernel<T, ELEM, D>, dim3(ctas), kThreads, Layout<D>::bytes, st, overlaps_previous(st), a);
+  const auto kernel = kv_attention_wide_kernel<T, ELEM, D>;
+  if (!allow_smem<id>(kernel, Layout<D>::bytes)) return set_error(MPSA_ERR_LAUNCH, "kv_attention: shared memory not granted");
+  launch_dependent(kernel, dim3(ctas), kThreads, Layout<D>::bytes, st, overlaps_previous(st), a);
   return check_launch("kv_attention");
 }
 template <typename T, int ELEM>

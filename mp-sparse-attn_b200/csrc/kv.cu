@@ -217,7 +217,8 @@ void append_lanes(const mpsa_kv_append_args& a, cudaStream_t st) {
   const bool many = (long long)a.T * a.cache.Hkv * a.B > 8ll * kAppendRows * rows * sm_count();
   const int per = many ? kAppendRows * rows : rows;
   const dim3 grid((a.T + per - 1) / per, a.cache.Hkv, a.B);
-  launch_dependent(many ? kv_append_kernel<T, ELEM, LANES, kAppendRows> : kv_append_kernel<T, ELEM, LANES, 1>, grid, kThreads, 0, st, overlaps_previous(st), a);
+  const auto kernel = many ? kv_append_kernel<T, ELEM, LANES, kAppendRows> : kv_append_kernel<T, ELEM, LANES, 1>;
+  launch_dependent(kernel, grid, kThreads, 0, st, overlaps_previous(st), a);
 }
 template <typename T, int ELEM>
 int append_as(const mpsa_kv_append_args& a, cudaStream_t st) {
@@ -234,7 +235,8 @@ template <typename T, int ELEM>
 int read_as(const mpsa_kv_read_args& a, cudaStream_t st) {
   const int rows = kThreads / (a.cache.D / 8) * kReadRows;
   const dim3 grid((a.max_len + rows - 1) / rows, a.cache.Hkv, a.B);
-  launch_dependent(a.cache.D == 64 ? kv_read_kernel<T, ELEM, 8, kReadRows> : kv_read_kernel<T, ELEM, 16, kReadRows>, grid, kThreads, 0, st, overlaps_previous(st), a);
+  const auto kernel = a.cache.D == 64 ? kv_read_kernel<T, ELEM, 8, kReadRows> : kv_read_kernel<T, ELEM, 16, kReadRows>;
+  launch_dependent(kernel, grid, kThreads, 0, st, overlaps_previous(st), a);
   return check_launch("kv_read");
 }
 template <typename T>

@@ -252,14 +252,16 @@ int launch(NormRope& a, cudaStream_t st) {
   if (a.norm == 2) {
     const int most = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
     const int threads = (most * LANES + 32 * kChunks - 1) / (32 * kChunks) * 32;
-    launch_dependent(norm_rope_across_kernel<T, W, LANES, INTERLEAVED>, dim3((unsigned)tokens, a.x[1] ? 2 : 1), threads, 0, st, overlaps_previous(st), a);
+    const auto kernel = norm_rope_across_kernel<T, W, LANES, INTERLEAVED>;
+    launch_dependent(kernel, dim3((unsigned)tokens, a.x[1] ? 2 : 1), threads, 0, st, overlaps_previous(st), a);
     return check_launch("norm_rope");
   }
   const long long groups = (tokens + kThreads / LANES - 1) / (kThreads / LANES);
   a.heads_per_cta = heads;                                           // split over CTAs where there are few tokens
   while (a.heads_per_cta > kAhead && groups * ((heads + a.heads_per_cta - 1) / a.heads_per_cta) < 8ll * sm_count()) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid((unsigned)groups, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
-  launch_dependent(norm_rope_heads_kernel<T, W, LANES, INTERLEAVED>, grid, kThreads, 0, st, overlaps_previous(st), a);
+  const auto kernel = norm_rope_heads_kernel<T, W, LANES, INTERLEAVED>;
+  launch_dependent(kernel, grid, kThreads, 0, st, overlaps_previous(st), a);
   return check_launch("norm_rope");
 }
 template <typename T, typename W>
