@@ -16,7 +16,9 @@
 //             score - 100, so that they stay finite (values below 2^-90 have fewer bits, then).
 // Fragments of K and V come from ldmatrix on the codes as they are (.trans for V: two keys of neighbouring depth elements in a register).
 //
-// It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each.
+// It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each.  8 KV heads of depth 128,
+// 4 query heads each: 32 sequences of up to 16384 tokens in E4M3 111 us (5.1 - 5.8 TB/s; 705 instructions a step and warp), 4 of 131072 in E2M1
+// 147 us (3.9 TB/s; ALU 62 %).  With queries in the M dimension the first took 140 us: half of each instruction's 16 rows were padding.
 #include "api_internal.h"
 #include "decode.cuh"
 
@@ -562,7 +564,8 @@ __global__ void __launch_bounds__(32 * kWarps, per_sm(NR, ELEM, D)) kv_attention
   }
 }
 
-// Units that several CTAs had a part of: a warp adds up one row's parts, in the order of the keys.
+// Units that several CTAs had a part of: a warp adds up one row's parts, in the order of the keys.  (Four rows a warp where units have 128, for a
+// quarter of the CTAs: trees of 32 tokens 181 us instead of 174.)
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_constant__ Call a, int ctas) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, units = a.cache.Hkv * a.groups;

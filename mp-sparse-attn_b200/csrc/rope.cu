@@ -1,4 +1,6 @@
 // RMS norm of queries and keys and their rotation by position in one pass (mpsa_norm_rope): every element is read once and written once.
+// Bound by HBM: 40 heads of 32768 tokens, each head's norm, 120 us (5.7 TB/s); 80 heads of 32760 tokens, norm across 40 heads, three axes,
+// 289 us (4.6 TB/s, issue 80 %).  A decoding step of 32 sequences takes the host's 7.8 us.
 #include "api_internal.h"
 #include "common.cuh"
 #include "serving.cuh"
@@ -105,7 +107,8 @@ __device__ __forceinline__ float squares(const float (&u)[4], const float (&v)[4
 }
 
 // Norm of each head, or none: D/8 lanes hold a row; they keep the token's angles for all of the CTA's heads, and the operand's weights.
-// kAhead rows are requested before the first is worked on.
+// kAhead rows are requested before the first is worked on.  Few heads a CTA where there are few tokens, all of them otherwise: four CTAs for a
+// token's 40 heads instead of one read its angles four times and took 154 us instead of 120.
 constexpr int kAhead = 4;
 template <typename T, typename W, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, 4) norm_rope_heads_kernel(const __grid_constant__ NormRope a) {

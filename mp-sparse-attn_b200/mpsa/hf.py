@@ -10,7 +10,8 @@ this, which needs no module surgery:
 
 What is routed to the kernel: calls without an explicit attention mask (or with the plain causal pattern the model
 announces through ``is_causal``), head_dim 64 or 128, more than one query token.  Everything else - decoding steps,
-padding masks, dropout, other head dims - goes to the library's own SDPA implementation, unchanged.
+padding masks, dropout, other head dims - goes to the library's own SDPA implementation, unchanged (a program that decodes over a quantised cache
+of its own calls mpsa.kv_cache_attention).
 """
 from typing import Optional
 
