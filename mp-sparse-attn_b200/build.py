@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "mpsa", "libmpsa.so")
 NATIVE_SRC = os.path.join(CSRC, "native.cpp")
+HEADER = os.path.join(os.path.dirname(HERE), "include", "mpsa.h")
 SOURCES = ["api.cu", "quant.cu", "prep.cu", "gemm.cu", "attn.cu", "route.cu", "attention.cu", "rope.cu", "kv.cu", "decode.cu", "decode_wide.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default", "--use_fast_math=false"]
@@ -34,7 +35,7 @@ def needs_build():
     for f in os.listdir(CSRC):
         if f != "native.cpp" and os.path.getmtime(os.path.join(CSRC, f)) > t:
             return True
-    return os.path.getmtime(__file__) > t
+    return max(os.path.getmtime(f) for f in (HEADER, __file__)) > t
 
 
 def build_lib(force=False, verbose=False):
@@ -76,8 +77,7 @@ def native_out():
 def build_native(force=False):
     """csrc/native.cpp -> native_out(), the module that takes torch tensors to the library (needs torch's headers)."""
     out = native_out()
-    header = os.path.join(os.path.dirname(HERE), "include", "mpsa.h")
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(f) for f in (NATIVE_SRC, header, __file__)):
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(f) for f in (NATIVE_SRC, HEADER, __file__)):
         return out
     import sysconfig
 
