@@ -13,7 +13,7 @@
 //             largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
 // One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
-// 8 sequences of up to 32768 tokens, 8 KV heads, trees of 32 tokens x 4 query heads: 156 - 180 us, 6300 cycles a step with two in flight on an SM:
+// 8 sequences of up to 32768 tokens, 8 KV heads, trees of 32 tokens x 4 query heads: 156 - 202 us by box, 6300 cycles a step with two in flight on an SM:
 // softmax 2300, P V 850, Q K^T 1500 (operands and conversion share the shared-memory pipe), the rest hand-overs and what the conversion is late.
 #include "api_internal.h"
 #include "decode.cuh"
