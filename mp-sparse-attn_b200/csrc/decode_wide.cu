@@ -8,7 +8,8 @@
 //             Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
 //   softmax   a thread a row: P times the largest scale of V of the 32 keys, rounded to fp16, goes over S; the reference U keeps that within
-//             fp16 as decode.cu says (there it is each block's own scale).  Steps in which every row sees every key are tried against the
+//             fp16 as decode.cu says (there it is each block's own scale).  The denominator adds up P itself: a key whose values are nothing,
+//             and whose product is, has its weight in it.  Steps in which every row sees every key are tried against the
 //             references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
 //             largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
@@ -68,6 +69,9 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
 }
 // 2^d in both halves (0 below 2^-24), d at most 0
 __device__ __forceinline__ uint32_t power2(int d) { return pack2(__half(), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23)); }
+
+// 2^e of a whole e, -126 at least
+__device__ __forceinline__ float power2f(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }
 
 // The parts of a unit that a CTA's run covers, one after the other, for each role alike.
 struct Run {
@@ -321,28 +325,27 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
           if (!special && __all_sync(0xffffffffu, U != -INFINITY)) {
             // as it is: products in registers, and over S if none has become too large
             uint32_t p[64], top = 0;
-            float now = l;
+            float sum = 0.0f, sum2 = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c], v = sh.v_size[par][c], ref = v - U;
-              float sum = 0.0f, sum2 = 0.0f;
+              const float f = rs * sh.k_size[par][c], v = power2f(sh.v_size[par][c]);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 float y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, ref));
+                for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -U));
                 sum += y[0] + y[1];
                 sum2 += y[2] + y[3];
                 uint32_t* const q = p + 16 * c + i / 2;
-                q[0] = pack2(__half(), y[0], y[1]);
-                q[1] = pack2(__half(), y[2], y[3]);
+                q[0] = pack2(__half(), y[0] * v, y[1] * v);
+                q[1] = pack2(__half(), y[2] * v, y[3] * v);
                 top = __vmaxu2(top, __vmaxu2(q[0], q[1]));
               }
-              now = fmaf(sum + sum2, exp2_fast(-v), now);
             }
+            const float now = l + (sum + sum2);
             // (a product of more than 2^15 is 0x7801 or more, an infinity or a NaN among them; none is negative)
             done = !__any_sync(0xffffffffu, __vcmpgtu2(top, 0x78007800u) != 0 || !(now < 0x1p115f));
             if (done) {
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32], p[16];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c], v = sh.v_size[par][c], at = v - ref;
+              const float f = rs * sh.k_size[par][c], v = power2f(sh.v_size[par][c]);
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
               float sum = 0.0f;
               tmem_ld_wait();
@@ -410,13 +413,13 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                 float y[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, at));
+                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -ref));
                   if (!(seen >> (i + e) & 1)) y[e] = 0.0f;
                 }
                 sum += y[0] + y[1];
-                p[i / 2] = pack2(__half(), y[0], y[1]);
+                p[i / 2] = pack2(__half(), y[0] * v, y[1] * v);
               }
-              l = fmaf(sum, exp2_fast(-v), l);
+              l += sum;
               tmem_st16(mine + 16 * c, p);
             }
           }
