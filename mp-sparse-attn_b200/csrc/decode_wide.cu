@@ -3,12 +3,14 @@
 //
 // A unit is up to 128 query rows, a step 128 keys.  Eight warps: 4 convert, 4 are the softmax, the first of which also issues the
 // tensor operations: what they wait for is what it has just done.
-//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory, relative to
-//             the largest scale of 32 keys of K or of V: what fp16 cannot hold is 2^-30 of the largest of those elements, E2M1 apart even less.
+//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory: K relative to
+//             the largest scale of 32 keys (a factor of the scores), V relative to the largest of its key (a factor of P).  What fp16 cannot
+//             hold is 2^-31 of the largest of those elements.
 //             Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
-//   softmax   a thread a row: P times the largest scale of V of the 32 keys, rounded to fp16, goes over S; the reference U keeps that within
-//             fp16 as decode.cu says (there it is each block's own scale).  The denominator adds up P itself: a key whose values are nothing,
+//   softmax   a thread a row: P times V's factor, rounded to fp16, goes over S; the reference U keeps that within fp16 as decode.cu says
+//             (there it is each block's own scale).  One factor for 32 keys was no faster, and took bits from all others where a key without
+//             weight had large values.  The denominator adds up P itself: a key whose values are nothing,
 //             and whose product is, has its weight in it.  Steps in which every row sees every key are tried against the
 //             references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
 //             largest one first.
@@ -40,7 +42,8 @@ struct Layout {
 struct Shared {
   uint64_t k_full, v_full, s_full, p_full, pv_done, q_full, drained;
   uint32_t tmem;
-  float k_size[2][4], v_size[2][4];                    // largest scale of 32 keys: of K, log2 of V's (two steps' worth, as below)
+  alignas(16) float v_size[2][128], v_log[2][128];     // each key's largest scale of V, and log2 of it (two steps' worth, as below)
+  float k_size[2][4];                                  // largest scale of K of 32 keys, in units of K's operand
   uint32_t there[2][4];                                // keys with a page and within the length
   uint32_t strange[2][4][4];                           // [32 keys][block of the depth]: scales of V that are NaN
 };
@@ -67,11 +70,11 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// 2^d in both halves (0 below 2^-24), d at most 0
+// What an element of the largest size becomes in an operand is 2^13 to 2^16: fp16 then goes as far down from it as it can.
+template <int ELEM> constexpr int kUp = ELEM == E4M3 ? 7 : ELEM == E5M2 ? 0 : 13;
+constexpr __host__ __device__ float down_by(int up) { return 1.0f / (float)(1 << up); }
+// 2^d in both halves (0 below 2^-24), d at most 15
 __device__ __forceinline__ uint32_t power2(int d) { return pack2(__half(), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23)); }
-
-// 2^e of a whole e, -126 at least
-__device__ __forceinline__ float power2f(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }
 
 // The parts of a unit that a CTA's run covers, one after the other, for each role alike.
 struct Run {
@@ -153,8 +156,8 @@ __device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, con
   }
 }
 
-// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by; base: the scale code that
-// stands for 1; nan: what a NaN scale becomes.
+// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by, negative ones by 2^-24 once
+// more; base: the scale code of key `lane` that stands for 2^kUp; nan: what a NaN scale becomes.
 template <int ELEM, int D>
 __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, uint32_t factors, int base, uint32_t nan, int lane) {
   using R = Rows<ELEM, D>;
@@ -163,7 +166,10 @@ __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, i
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const uint32_t e = r.scale >> (8 * i) & 255u;
-    f[i] = e == 255u ? nan : power2((int)e - base);
+    const int d = (int)e - base + kUp<ELEM>;
+    f[i] = e == 255u ? nan : power2(d);
+    if constexpr (ELEM == E5M2)                        // (codes reach 2^16: the factor would be nothing where the product is not yet)
+      if (e != 255u && d < -24) f[i] = power2(d + 24) | 0x80008000u;
   }
   __syncwarp();
   store_shared16(factors + 16 * lane, f[0], f[1], f[2], f[3]);
@@ -189,7 +195,13 @@ __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, i
         elem_two<ELEM>(w[2 * j], x[0], x[1]);
         elem_two<ELEM>(w[2 * j + 1], x[2], x[3]);
       }
-      store_shared16((first ^ (16 * j + (R::rpi == 4 ? i % 2 * 64 : 0))) + i * R::rpi * 128, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[y] = times(x[y], m);
+      if constexpr (ELEM == E5M2)
+        if (m & 0x8000u)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[y] = times(x[y], 0x80018001u);          // -2^-24
+      store_shared16((first ^ (16 * j + (R::rpi == 4 ? i % 2 * 64 : 0))) + i * R::rpi * 128, x[0], x[1], x[2], x[3]);
     }
   }
 }
@@ -330,7 +342,8 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c], v = power2f(sh.v_size[par][c]);
+              const float f = rs * sh.k_size[par][c];
+              const float* const vs = &sh.v_size[par][32 * c];
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -339,9 +352,10 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                 for (int e = 0; e < 4; ++e) y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -U));
                 sum += y[0] + y[1];
                 sum2 += y[2] + y[3];
+                const float4 v = *reinterpret_cast<const float4*>(vs + i);
                 uint32_t* const q = p + 16 * c + i / 2;
-                q[0] = pack2(__half(), y[0] * v, y[1] * v);
-                q[1] = pack2(__half(), y[2] * v, y[3] * v);
+                q[0] = pack2(__half(), y[0] * v.x, y[1] * v.y);
+                q[1] = pack2(__half(), y[2] * v.z, y[3] * v.w);
                 top = __vmaxu2(top, __vmaxu2(q[0], q[1]));
               }
             }
@@ -372,12 +386,12 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c], v = fmaxf(sh.v_size[par][c], kLeast);
+              const float f = rs * sh.k_size[par][c];
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float y = fmaf(__uint_as_float(x[i]), f, v);
+                const float y = fmaf(__uint_as_float(x[i]), f, sh.v_log[par][32 * c + i]);
                 top = fmaxf(top, seen >> i & 1 ? y : -INFINITY);
               }
             }
@@ -404,7 +418,8 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32], p[16];
               tmem_ld32(mine + 32 * c, x);
-              const float f = rs * sh.k_size[par][c], v = power2f(sh.v_size[par][c]);
+              const float f = rs * sh.k_size[par][c];
+              const float* const vs = &sh.v_size[par][32 * c];
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
               float sum = 0.0f;
               tmem_ld_wait();
@@ -417,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                   if (!(seen >> (i + e) & 1)) y[e] = 0.0f;
                 }
                 sum += y[0] + y[1];
-                p[i / 2] = pack2(__half(), y[0] * v, y[1] * v);
+                p[i / 2] = pack2(__half(), y[0] * vs[i], y[1] * vs[i + 1]);
               }
               l += sum;
               tmem_st16(mine + 16 * c, p);
@@ -461,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
       const bool whole = run.s0 == 0 && run.s1 == run.steps;
       const long long slot = (2ll * blockIdx.x + (run.s0 == 0)) * kWideRows + warp * 32 + lane;
       const bool none = l == 0.0f || tok >= run.ql;
-      const float w = !whole ? 1.0f : none ? 0.0f : 1.0f / l;
+      const float w = !whole ? down_by(kUp<ELEM>) : none ? 0.0f : down_by(kUp<ELEM>) / l;
       T* const y = static_cast<T*>(a.out) + (run.now * a.o_sb + hq * a.o_sh + (long long)tok * a.o_sl);
 #pragma unroll 1
       for (int i = 0; i < D / 16; ++i) {
@@ -541,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
       look_up();
       if (now) {
         if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
-        // one reference for the warp's keys of K, and one for V
+        // one reference for the warp's keys of K; one for each key of V: what one row sees of no weight, or not at all, may be large to another
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -552,13 +567,13 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
           if (lane == 0) sh.strange[par][w][i] = strange;
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        vtop = __reduce_max_sync(0xffffffffu, max(vtop, 1u));
+        sh.v_size[par][32 * w + lane] = scale_value(vtop);
+        sh.v_log[par][32 * w + lane] = fmaxf((float)((int)vtop - 127), kLeast);
         convert<ELEM, D>(k, kt, 32 * w, factors, (int)top, 0x7fff7fffu, lane);
         const uint32_t has = __ballot_sync(0xffffffffu, here);
         if (lane == 0) {
           sh.there[par][w] = has;
-          sh.k_size[par][w] = scale_value(top);
-          sh.v_size[par][w] = (float)((int)vtop - 127);
+          sh.k_size[par][w] = scale_value(top) * down_by(kUp<ELEM>);
         }
         fence_proxy_async_smem();
         mbar_arrive(&sh.k_full);

@@ -52,3 +52,70 @@ def test_keys_without_values_keep_their_weight(elem, gap, T, place, written):
     sm = gap / 4.0 / math.log2(math.e)
     out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), sm_scale=sm, return_lse=True)
     check_attention(c, table, [n], q, out.cpu(), lse.cpu(), sm=sm)
+
+
+@pytest.mark.parametrize("octaves", [16, 26, 40, 60])
+@pytest.mark.parametrize("T", [6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_large_values_of_keys_that_a_row_does_not_see(elem, T, octaves):
+    """A drafted token's values are larger than all others' by far: the drafts that do not see it have the same result as without it, over few keys
+    and over many."""
+    import mpsa
+    g = torch.Generator().manual_seed(octaves)
+    D, Hq, Hkv = 64, 2, 1
+    for n in (T + 90, 32768 + T):
+        k, v = rnd(g, 1, Hkv, n, D), rnd(g, 1, Hkv, n, D)
+        v[:, :, n - T + 2] *= 2.0 ** octaves
+        c, table = cache_of_rows(g, k, v, elem)
+        q = rnd(g, 1, Hq, T, D)
+        mask = tree_mask(g, T)
+        mask[:, 2] = False
+        mask[2, 2] = True
+        args = (q.cuda(), c, table.cuda(), i32(n))
+        out, lse = mpsa.kv_cache_attention(*args, mask=mask.cuda(), return_lse=True)
+        check_attention(c, table, [n], q, out.cpu(), lse.cpu(), mask=mask)
+
+
+@pytest.mark.parametrize("place", [3, 700])
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_large_values_of_improbable_keys(elem, T, place):
+    """A key whose score is 120 below the others' in log2 has values that are 2^60 larger: with its weight it is nothing, and it takes nothing from
+    the keys beside it."""
+    import mpsa
+    g = torch.Generator().manual_seed(place)
+    n, D, Hq = 1000, 64, 4
+    k, v = rnd(g, 1, 1, n, D), rnd(g, 1, 1, n, D)
+    k[..., 0] = 0.0
+    k[:, :, place] = 0.0
+    k[:, :, place, 0] = -16.0
+    v[:, :, place] *= 2.0 ** 60
+    q = rnd(g, 1, Hq, T, D)
+    q[..., 0] = 120.0 / 16.0 / math.log2(math.e) * 8.0 * 1.01
+    c, table = cache_of_rows(g, k, v, elem)
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+    check_attention(c, table, [n], q, out.cpu(), lse.cpu())
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_a_block_of_a_key_that_is_larger_than_its_others(elem, T):
+    """All keys' values are 2^26 larger in their first 32 depth elements: the others keep the bits that 2^-32 of a key's largest product leaves."""
+    import mpsa
+    g = torch.Generator().manual_seed(5)
+    n, D, Hq = 700, 128, 4
+    k, v = rnd(g, 1, 1, n, D), 1.0 + torch.rand(1, 1, n, D, generator=g)
+    v[..., :32] *= 2.0 ** 26
+    c, table = cache_of_rows(g, k, v.to(BF16), elem)
+    q = rnd(g, 1, Hq, T, D, amp=0.1)
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+    check_attention(c, table, [n], q, out.cpu(), lse.cpu())
+    k, v = (P.values(P.gather(getattr(c, x), table[0], n), P.gather(getattr(c, x + "_scale"), table[0], n), elem) for x in ("k", "v"))
+    # P times the block's scale and, with many rows, the element in units of its key's largest are held to 2^-25 of what is 2^7 for the largest
+    # product of the row: 2^-32 of it each, and at most twice that with elements of up to twice the others in size; of 700 keys at most
+    seen = torch.ones(T, n, dtype=torch.bool)
+    seen[:, n - T:] = torch.ones(T, T).tril().bool()
+    o, _, a, _, big = P.attention(q[0].double(), k, v, seen, D ** -0.5)
+    err = (out[0].cpu().double() - o).abs()[..., 32:]
+    tol = (half_step(BF16) * o.abs() * 1.01 + 2.0 ** -10 * a + n * 2.0 ** -30 * big.unsqueeze(-1))[..., 32:]
+    assert bool((err <= tol).all()), float((err / tol).max())
