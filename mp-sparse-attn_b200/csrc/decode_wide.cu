@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
 #pragma unroll
               for (int c = 0; c < 4; ++c) vis[c] = seen_keys(mk, pos + 32 * c - run.first, live ? tok : a.T, run.ql) & sh.there[par][c];
             }
-            // the largest product
+            // The largest product.  Scores are rounded before anything is added to them, here and below: the largest one must come out as the same
+            // number, as where U is large, what a fused product keeps in its last bits is more than all a weight can be.
             float top = -INFINITY;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float y = fmaf(__uint_as_float(x[i]), f, sh.v_log[par][32 * c + i]);
+                const float y = __fmul_rn(__uint_as_float(x[i]), f) + sh.v_log[par][32 * c + i];
                 top = fmaxf(top, seen >> i & 1 ? y : -INFINITY);
               }
             }
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                 float y[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  y[e] = exp2_fast(fmaf(__uint_as_float(x[i + e]), f, -ref));
+                  y[e] = exp2_fast(__fmul_rn(__uint_as_float(x[i + e]), f) - ref);
                   if (!(seen >> (i + e) & 1)) y[e] = 0.0f;
                 }
                 sum += y[0] + y[1];

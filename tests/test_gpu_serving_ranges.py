@@ -119,3 +119,32 @@ def test_a_block_of_a_key_that_is_larger_than_its_others(elem, T):
     err = (out[0].cpu().double() - o).abs()[..., 32:]
     tol = (half_step(BF16) * o.abs() * 1.01 + 2.0 ** -10 * a + n * 2.0 ** -30 * big.unsqueeze(-1))[..., 32:]
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("octaves", [10, 24, 27, 32, 40, 60, 100])
+@pytest.mark.parametrize("T", [1, 6, 40])
+def test_scores_of_any_size(T, octaves, sign):
+    """Scores so large that neighbouring fp32 numbers are further apart than the logarithms of two weights: the largest key has all the weight, and
+    the row is not empty.  Keys have one element and differ by an eighth at least, so that the largest one is so in any rounding."""
+    import mpsa
+    g = torch.Generator().manual_seed(octaves)
+    n, D, Hq = 700, 64, 4
+    k, v = torch.zeros(1, 1, n, D), rnd(g, 1, 1, n, D)
+    size = torch.randint(2, 9, (n,), generator=g).float() / 16
+    size[n - T] = size[0] = size[320] = 0.25                   # (what the first draft sees at the least, and what is seen with it)
+    best = 333
+    size[best] = 0.625 if sign > 0 else 0.0625
+    k[0, 0, :, 0] = size * sign
+    q = rnd(g, 1, Hq, T, D)
+    q[..., 0] = 1.40625 * 2.0 ** octaves
+    c, table = cache_of_rows(g, k.to(BF16), v, "e4m3")
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+    if octaves == 10:                                          # (scores that still matter)
+        check_attention(c, table, [n], q, out.cpu(), lse.cpu())
+        return
+    held = P.values(P.gather(c.v, table[0], n), P.gather(c.v_scale, table[0], n), "e4m3")[0, best]
+    # the weight of the one key is exactly 1 where all others' are 0: P is a power of two then or has its rounding to fp16, 2^-11
+    assert bool(((out[0].cpu().double() - held).abs() <= (half_step(BF16) * 1.01 + 2.0 ** -11) * held.abs() + 2.0 ** -24).all())
+    s = 1.40625 * 2.0 ** octaves * float(k[0, 0, best, 0]) * D ** -0.5 * math.log2(math.e)
+    assert bool(((lse.cpu().double() - s).abs() <= 2.0 ** -20 * abs(s) + 2.0 ** -16).all())
