@@ -3,16 +3,16 @@
 //
 // A unit is up to 128 query rows, a step 128 keys.  Eight warps: 4 convert, 4 are the softmax, the first of which also issues the
 // tensor operations: what they wait for is what it has just done.
-//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory: K relative to
-//             the largest scale of 32 keys (a factor of the scores), V relative to the largest of its key (a factor of P).  What fp16 cannot
-//             hold is 2^-31 of the largest of those elements.
+//   convert   the codes of a step's keys and values, kept on their way in registers one step ahead, become fp16 in shared memory: V relative to
+//             the largest scale of its key (a factor of P), K to the largest of 32 keys (a factor of the scores) where their scales are so near
+//             that all codes are exact, and otherwise to its key's too.  What fp16 cannot hold is 2^-31 of the key's largest element.
 //             Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
 //   softmax   a thread a row: P times V's factor, rounded to fp16, goes over S; the reference U keeps that within fp16 as decode.cu says
 //             (there it is each block's own scale).  One factor for 32 keys was no faster, and took bits from all others where a key without
 //             weight had large values.  The denominator adds up P itself: a key whose values are nothing,
-//             and whose product is, has its weight in it.  Steps in which every row sees every key are tried against the
-//             references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
+//             and whose product is, has its weight in it.  Steps in which every row sees every key (and K is alike) are tried against
+//             the references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
 //             largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
 // One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
@@ -44,6 +44,9 @@ struct Shared {
   uint32_t tmem;
   alignas(16) float v_size[2][128], v_log[2][128];     // each key's largest scale of V, and log2 of it (two steps' worth, as below)
   float k_size[2][4];                                  // largest scale of K of 32 keys, in units of K's operand
+  float k_part[2][128];                                // where these keys differ by more than kSpread: each key's largest scale as part of it
+  uint32_t uneven[2][4];
+  alignas(4) uint8_t odd[2][4];                        // uneven, or not all there
   uint32_t there[2][4];                                // keys with a page and within the length
   uint32_t strange[2][4][4];                           // [32 keys][block of the depth]: scales of V that are NaN
 };
@@ -72,6 +75,8 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
 }
 // What an element of the largest size becomes in an operand is 2^13 to 2^16: fp16 then goes as far down from it as it can.
 template <int ELEM> constexpr int kUp = ELEM == E4M3 ? 7 : ELEM == E5M2 ? 0 : 13;
+// Octaves that scales of K of 32 keys may differ by: all element codes are exact in the operand then.
+template <int ELEM> constexpr int kSpread = ELEM == E4M3 ? 22 : ELEM == E5M2 ? 8 : 36;
 constexpr __host__ __device__ float down_by(int up) { return 1.0f / (float)(1 << up); }
 // 2^d in both halves (0 below 2^-24), d at most 15
 __device__ __forceinline__ uint32_t power2(int d) { return pack2(__half(), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23), __uint_as_float((uint32_t)(max(d, -40) + 127) << 23)); }
@@ -332,7 +337,14 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
         const int par = n & 1, pos = s * kWideStep;
         if (busy) {
           const bool special = pos + kWideStep > (a.T > 1 || a.mask ? run.first : run.len) ||
-                               (sh.there[par][0] & sh.there[par][1] & sh.there[par][2] & sh.there[par][3]) != 0xffffffffu;
+                               *reinterpret_cast<const uint32_t*>(sh.odd[par]) != 0u;
+          auto scores = [&](int c, uint32_t (&x)[32]) { // of 32 keys, in units of the largest
+            tmem_ld32(mine + 32 * c, x);
+            tmem_ld_wait();
+            if (sh.uneven[par][c])
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * sh.k_part[par][32 * c + i]);
+          };
           bool done = false;
           if (!special && __all_sync(0xffffffffu, U != -INFINITY)) {
             // as it is: products in registers, and over S if none has become too large
@@ -386,10 +398,9 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32];
-              tmem_ld32(mine + 32 * c, x);
+              scores(c, x);
               const float f = rs * sh.k_size[par][c];
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
-              tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float y = __fmul_rn(__uint_as_float(x[i]), f) + sh.v_log[par][32 * c + i];
@@ -418,12 +429,11 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t x[32], p[16];
-              tmem_ld32(mine + 32 * c, x);
+              scores(c, x);
               const float f = rs * sh.k_size[par][c];
               const float* const vs = &sh.v_size[par][32 * c];
               const uint32_t seen = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
               float sum = 0.0f;
-              tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
                 float y[2];
@@ -557,23 +567,31 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
       look_up();
       if (now) {
         if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
-        // one reference for the warp's keys of K; one for each key of V: what one row sees of no weight, or not at all, may be large to another
-        uint32_t top = 0;
+        // One reference for the warp's keys of K where they are alike, one for each key of V, and for each of K otherwise: a key that a row
+        // does not see, or gives no weight, may be larger than the rest by far.  (Codes 0 and 1 are blocks of nothing: no element reaches 2^-110.)
+        uint32_t top = 0, low = 255;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const uint32_t e = k.scale >> (8 * i) & 255u, d = v.scale >> (8 * i) & 255u;
           top = max(top, e == 255u ? 0u : e);
+          low = min(low, e < 2u ? 255u : e);
           vtop = max(vtop, d == 255u ? 0u : d);
           const uint32_t strange = __ballot_sync(0xffffffffu, d == 255u);
           if (lane == 0) sh.strange[par][w][i] = strange;
         }
+        const uint32_t own = top;
         top = __reduce_max_sync(0xffffffffu, top);
+        low = __reduce_min_sync(0xffffffffu, low);
+        const bool uneven = (int)top - (int)low > kSpread<ELEM>;
+        if (uneven) sh.k_part[par][32 * w + lane] = __uint_as_float((uint32_t)max(127 - (int)(top - own), 0) << 23);
         sh.v_size[par][32 * w + lane] = scale_value(vtop);
         sh.v_log[par][32 * w + lane] = fmaxf((float)((int)vtop - 127), kLeast);
-        convert<ELEM, D>(k, kt, 32 * w, factors, (int)top, 0x7fff7fffu, lane);
+        convert<ELEM, D>(k, kt, 32 * w, factors, (int)(uneven ? own : top), 0x7fff7fffu, lane);
         const uint32_t has = __ballot_sync(0xffffffffu, here);
         if (lane == 0) {
           sh.there[par][w] = has;
+          sh.uneven[par][w] = uneven;
+          sh.odd[par][w] = uneven || has != 0xffffffffu;
           sh.k_size[par][w] = scale_value(top) * down_by(kUp<ELEM>);
         }
         fence_proxy_async_smem();

@@ -148,3 +148,91 @@ def test_scores_of_any_size(T, octaves, sign):
     assert bool(((out[0].cpu().double() - held).abs() <= (half_step(BF16) * 1.01 + 2.0 ** -11) * held.abs() + 2.0 ** -24).all())
     s = 1.40625 * 2.0 ** octaves * float(k[0, 0, best, 0]) * D ** -0.5 * math.log2(math.e)
     assert bool(((lse.cpu().double() - s).abs() <= 2.0 ** -20 * abs(s) + 2.0 ** -16).all())
+
+
+def check_by_key(c, table, n, q, out, lse, mask=None):
+    """As check_attention for one sequence, with each key's score held to its own size.
+
+    Score j is off by (D + 8) 2^-23 of the sum of its own terms' magnitudes, and by what an operand cannot hold: 2^-31 of the key's largest element and
+    2^-25 of the row's largest query element in each term.  That moves P_j by a factor exp(d_j); out = sum P v / sum P then moves by at most
+    sum |dP_j| (|v_j| + |out|) / sum P.  The rest is check_attention's."""
+    T, D = q.shape[2], q.shape[3]
+    G = q.shape[1] // c.num_kv_heads
+    k, v = (P.values(P.gather(getattr(c, x), table[0], n), P.gather(getattr(c, x + "_scale"), table[0], n), c.elem).repeat_interleave(G, 0) for x in ("k", "v"))
+    seen = torch.ones(T, n, dtype=torch.bool)
+    seen[:, n - T:] = torch.ones(T, T).tril().bool() if mask is None else mask
+    x, sm = q[0].double(), D ** -0.5
+    s = torch.where(seen, x @ k.transpose(1, 2) * sm, float("-inf"))
+    d = (D + 8) * 2.0 ** -23 * (x.abs() @ k.abs().transpose(1, 2)) + 2.0 ** -31 * x.abs().sum(-1, keepdim=True) * k.abs().amax(-1).unsqueeze(1)
+    d = (d + 2.0 ** -25 * x.abs().amax(-1, keepdim=True) * k.abs().sum(-1).unsqueeze(1)) * sm + 2.0 ** -22
+    l = torch.logsumexp(s, -1, keepdim=True)
+    p = torch.exp(s - l)
+    move = torch.where(seen, torch.exp(torch.minimum(s - l + d, torch.tensor(700.0, dtype=torch.float64))) - p, 0.0)
+    o, a = p @ v, p @ v.abs()
+    got, gl = out[0].double(), lse[0].double()
+    tol = half_step(q.dtype) * o.abs() * 1.01 + (2.0 ** -11 + 2.0 ** -16) * a + 1.01 * (move @ v.abs() + o.abs() * move.sum(-1, keepdim=True))
+    tol = tol + n * 2.0 ** -31 * (p * v.abs().amax(-1).unsqueeze(1)).amax(-1, keepdim=True) + 2.0 ** -24
+    assert bool(((got - o).abs() <= tol).all()), float(((got - o).abs() / tol).max())
+    l = l.squeeze(-1) * math.log2(math.e)
+    assert bool(((gl - l).abs() <= torch.log2(1 + move.sum(-1)) * 1.01 + 2.0 ** -16 + 2.0 ** -23 * l.abs()).all())
+    return float((tol < 0.1 * a + 1e-3).double().mean())       # (where a score is held to less than a bit nothing is tested)
+
+
+@pytest.mark.parametrize("octaves", [12, 26, 40, 60])
+@pytest.mark.parametrize("T", [6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_large_keys_that_a_row_does_not_see(elem, T, octaves):
+    import mpsa
+    g = torch.Generator().manual_seed(octaves + 1)
+    D, Hq, Hkv, n = 64, 4, 2, T + 90
+    k, v = rnd(g, 1, Hkv, n, D), rnd(g, 1, Hkv, n, D)
+    k[:, :, n - T + 2] *= 2.0 ** octaves
+    c, table = cache_of_rows(g, k, v, elem)
+    q = rnd(g, 1, Hq, T, D)
+    mask = tree_mask(g, T)
+    mask[:, 2] = False
+    mask[2, 2] = True
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), mask=mask.cuda(), return_lse=True)
+    keep = [t for t in range(T) if t != 2]                     # (the draft itself: a softmax of one key, or of all but it)
+    check_by_key(c, table, n, q, out.cpu(), lse.cpu(), mask)
+    only = torch.ones(T, n, dtype=torch.bool)
+    only[:, n - T:] = mask
+    k, v = (P.values(P.gather(getattr(c, x), table[0], n), P.gather(getattr(c, x + "_scale"), table[0], n), elem) for x in ("k", "v"))
+    o, _, a, mag, big = P.attention(q[0].double(), k, v, only, D ** -0.5)
+    tol = half_step(BF16) * o.abs() * 1.01 + (2 * ((D + 8) * 2.0 ** -23 * mag.unsqueeze(-1) + 2.0 ** -22) + 2.0 ** -11 + 2.0 ** -16) * a + n * 2.0 ** -31 * big.unsqueeze(-1) + 2.0 ** -24
+    assert bool(((out[0].cpu().double() - o).abs() <= tol)[:, keep].all())
+
+
+@pytest.mark.parametrize("octaves", [12, 26, 60])
+@pytest.mark.parametrize("place", [3, 700])
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_large_keys_without_weight(elem, T, place, octaves):
+    """A key that is larger than the others by far, against the queries: its weight is nothing, and the others' scores are their own."""
+    import mpsa
+    g = torch.Generator().manual_seed(place)
+    n, D, Hq = 1000, 64, 4
+    k, v = rnd(g, 1, 1, n, D), rnd(g, 1, 1, n, D)
+    k[..., 0] = 0.0
+    k[:, :, place] = 0.0
+    k[:, :, place, 0] = -2.0 ** octaves
+    q = rnd(g, 1, Hq, T, D)
+    q[..., 0] = 4.0
+    c, table = cache_of_rows(g, k, v, elem)
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+    assert check_by_key(c, table, n, q, out.cpu(), lse.cpu()) > 0.99
+
+
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_keys_and_values_of_all_sizes(elem, T):
+    """Keys from 2^-40 to 2^8 and values from 2^-30 to 2^30 of the usual, side by side; drafts that see few of them among them."""
+    import mpsa
+    g = torch.Generator().manual_seed(T)
+    D, Hq, n = 128, 2, 900
+    k = rnd(g, 1, 1, n, D, dtype=FP32) * torch.exp2(torch.randint(-40, 9, (1, 1, n, 1), generator=g).float()) * 2.0 ** -6
+    v = rnd(g, 1, 1, n, D, dtype=FP32) * torch.exp2(torch.randint(-30, 31, (1, 1, n, 1), generator=g).float())
+    c, table = cache_of_rows(g, k, v, elem)
+    q = rnd(g, 1, Hq, T, D)
+    out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+    check_by_key(c, table, n, q, out.cpu(), lse.cpu())
