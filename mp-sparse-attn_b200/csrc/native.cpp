@@ -287,8 +287,23 @@ bool page_table(const at::Tensor& t, int64_t B, int device) {
   return t.dim() == 2 && t.size(0) == B && fits_int(t.size(1)) && t.scalar_type() == at::kInt && t.stride(1) == 1 && t.get_device() == device;
 }
 
-const mpsa_kv_cache* cache_of(PyObject* o) {
-  return PyBytes_CheckExact(o) && PyBytes_GET_SIZE(o) == sizeof(mpsa_kv_cache) ? reinterpret_cast<const mpsa_kv_cache*>(PyBytes_AS_STRING(o)) : nullptr;
+// The argument block of a cache (block, k, k_scale, v, v_scale) if it is that of its buffers as they are now; own: the first of them.
+const mpsa_kv_cache* cache_of(PyObject* o, const at::Tensor*& own) {
+  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 5 || !PyBytes_CheckExact(PyTuple_GET_ITEM(o, 0)) ||
+      PyBytes_GET_SIZE(PyTuple_GET_ITEM(o, 0)) != sizeof(mpsa_kv_cache) || !(own = plain(PyTuple_GET_ITEM(o, 1))))
+    return nullptr;
+  const mpsa_kv_cache* const c = reinterpret_cast<const mpsa_kv_cache*>(PyBytes_AS_STRING(PyTuple_GET_ITEM(o, 0)));
+  const void* const at[4] = {c->k, c->k_scale, c->v, c->v_scale};
+  const int64_t row[2] = {c->elem == 2 ? c->D / 2 : c->D, c->D / 32};
+  for (int i = 0; i < 4; ++i) {
+    PyObject* const x = PyTuple_GET_ITEM(o, 1 + i);
+    if (!THPVariable_CheckExact(x)) return nullptr;
+    const c10::TensorImpl* const t = THPVariable_Unpack(x).unsafeGetTensorImpl();
+    if (!t->has_storage() || t->data() != at[i] || t->dim() != 4 || !t->is_contiguous()) return nullptr;     // (the address is the device's, too)
+    const auto z = t->sizes();
+    if (z[0] != c->num_pages || z[1] != c->Hkv || z[2] != c->page_size || z[3] != row[i & 1]) return nullptr;
+  }
+  return c;
 }
 
 // kv_cache(k, k_scale, v, v_scale, elem) -> the cache's argument block as bytes
@@ -398,14 +413,15 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// kv_append(cache, cache_k, k, v, page_table, start, counts, hnd) -> error code
+// kv_append(cache, k, v, page_table, start, counts, hnd) -> error code
 PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!counted(n, 8, "kv_append")) return nullptr;
+  if (!counted(n, 7, "kv_append")) return nullptr;
   return guarded([&]() -> PyObject* {
-    const mpsa_kv_cache* cache = cache_of(a[0]);
-    const at::Tensor *own = plain(a[1]), *k = plain(a[2]), *v = plain(a[3]), *table = plain(a[4]), *start = plain(a[5]), *counts;
-    if (!cache || !own || !k || !v || !table || !start || !optional_plain(a[6], counts)) Py_RETURN_NONE;
-    const int hnd = PyObject_IsTrue(a[7]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
+    const at::Tensor* own;
+    const mpsa_kv_cache* cache = cache_of(a[0], own);
+    const at::Tensor *k = plain(a[1]), *v = plain(a[2]), *table = plain(a[3]), *start = plain(a[4]), *counts;
+    if (!cache || !k || !v || !table || !start || !optional_plain(a[5], counts)) Py_RETURN_NONE;
+    const int hnd = PyObject_IsTrue(a[6]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
     if (!rows_aligned(*k, 8) || !rows_aligned(*v, 8) || asks_gradient(*k) || asks_gradient(*v) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || any_dtype(*k) < 0 ||
         k->get_device() != device || v->get_device() != device || k->size(h) != cache->Hkv || k->size(3) != cache->D)
       Py_RETURN_NONE;
@@ -431,15 +447,16 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// kv_read(cache, cache_k, page_table, lengths, max_len, out_dtype) -> (k, v)
+// kv_read(cache, page_table, lengths, max_len, out_dtype) -> (k, v)
 PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!counted(n, 6, "kv_read")) return nullptr;
+  if (!counted(n, 5, "kv_read")) return nullptr;
   return guarded([&]() -> PyObject* {
-    const mpsa_kv_cache* cache = cache_of(a[0]);
-    const at::Tensor *own = plain(a[1]), *table = plain(a[2]), *lengths = plain(a[3]);
-    const long long len = as_ll(a[4]), type = as_ll(a[5]);
+    const at::Tensor* own;
+    const mpsa_kv_cache* cache = cache_of(a[0], own);
+    const at::Tensor *table = plain(a[1]), *lengths = plain(a[2]);
+    const long long len = as_ll(a[3]), type = as_ll(a[4]);
     if (PyErr_Occurred()) return nullptr;
-    if (!cache || !own || !table || !lengths || !fits_int(len) || type < 0 || type > 2 || table->dim() != 2) Py_RETURN_NONE;
+    if (!cache || !table || !lengths || !fits_int(len) || type < 0 || type > 2 || table->dim() != 2) Py_RETURN_NONE;
     const int64_t B = table->size(0);
     if (!fits_int(B) || !page_table(*table, B, own->get_device()) || !indices(*lengths, B, own->get_device())) Py_RETURN_NONE;
     mpsa_kv_read_args c = {};
@@ -463,17 +480,18 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// kv_attention(cache, cache_k, q, page_table, lengths, q_lens, mask, status, sm_scale, want_lse, hnd) -> out or (out, lse)
+// kv_attention(cache, q, page_table, lengths, q_lens, mask, status, sm_scale, want_lse, hnd) -> out or (out, lse)
 PyObject* kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!counted(n, 11, "kv_attention")) return nullptr;
+  if (!counted(n, 10, "kv_attention")) return nullptr;
   return guarded([&]() -> PyObject* {
-    const mpsa_kv_cache* cache = cache_of(a[0]);
-    const at::Tensor *own = plain(a[1]), *q = plain(a[2]), *table = plain(a[3]), *lengths = plain(a[4]), *qlens, *mask;
-    if (!cache || !own || !q || !table || !lengths || !optional_plain(a[5], qlens) || !optional_plain(a[6], mask)) Py_RETURN_NONE;
+    const at::Tensor* own;
+    const mpsa_kv_cache* cache = cache_of(a[0], own);
+    const at::Tensor *q = plain(a[1]), *table = plain(a[2]), *lengths = plain(a[3]), *qlens, *mask;
+    if (!cache || !q || !table || !lengths || !optional_plain(a[4], qlens) || !optional_plain(a[5], mask)) Py_RETURN_NONE;
     mpsa_kv_attention_args c = {};
-    c.status = static_cast<int*>(PyLong_AsVoidPtr(a[7]));
-    c.sm_scale = (float)PyFloat_AsDouble(a[8]);
-    const int lse = PyObject_IsTrue(a[9]), hnd = PyObject_IsTrue(a[10]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
+    c.status = static_cast<int*>(PyLong_AsVoidPtr(a[6]));
+    c.sm_scale = (float)PyFloat_AsDouble(a[7]);
+    const int lse = PyObject_IsTrue(a[8]), hnd = PyObject_IsTrue(a[9]), h = hnd ? 1 : 2, l = hnd ? 2 : 1, device = own->get_device();
     if (PyErr_Occurred()) return nullptr;
     c.dtype = in_dtype(*q);
     if (c.dtype < 0 || !rows_aligned(*q, 8) || asks_gradient(*q) || q->get_device() != device || q->size(3) != cache->D || q->size(h) % cache->Hkv || q->size(l) > 1024) Py_RETURN_NONE;

@@ -181,22 +181,25 @@ class KVCache:
     elem: str = "e4m3"
 
     def __post_init__(self):
+        """The argument block of the buffers as they are now, beside them.  The short way compares the two at every call and leaves it to the long
+        way, which comes here again, where they differ: a program may have exchanged a buffer's memory."""
         if self.elem not in _ELEM:
             raise ValueError(f"unknown cache element {self.elem!r}")
-        block = _lib.native().kv_cache(self.k, self.k_scale, self.v, self.v_scale, _ELEM[self.elem])         # the argument block, as bytes
-        if block is not None:
-            object.__setattr__(self, "_c", block)
-            return
-        _require_cuda(self.k, self.v, self.k_scale, self.v_scale)
-        if self.k.dim() != 4:
-            raise ValueError("cache codes must be [pages, heads, page size, bytes]")
-        pages, heads, page, row = self.k.shape
-        D = row * 2 if self.elem == "e2m1" else row
-        for t, n in ((self.k, row), (self.v, row), (self.k_scale, D // 32), (self.v_scale, D // 32)):
-            if t.dtype is not torch.uint8 or t.shape != (pages, heads, page, n) or not t.is_contiguous() or t.device != self.k.device:
-                raise ValueError("cache buffers must be contiguous uint8 [pages, heads, page size, ...] on one device")
-        object.__setattr__(self, "_c", bytes(_Cache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), pages,
-                                                    page, heads, D, _ELEM[self.elem])))
+        block = _lib.native().kv_cache(k := self.k, ks := self.k_scale, v := self.v, vs := self.v_scale, e := _ELEM[self.elem])         # as bytes
+        if block is None:
+            _require_cuda(k, v, ks, vs)
+            if k.dim() != 4:
+                raise ValueError("cache codes must be [pages, heads, page size, bytes]")
+            pages, heads, page, row = k.shape
+            D = row * 2 if self.elem == "e2m1" else row
+            for t, n in ((k, row), (v, row), (ks, D // 32), (vs, D // 32)):
+                if t.dtype is not torch.uint8 or t.shape != (pages, heads, page, n) or not t.is_contiguous() or t.device != k.device:
+                    raise ValueError("cache buffers must be contiguous uint8 [pages, heads, page size, ...] on one device")
+            block = bytes(_Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, page, heads, D, e))
+        object.__setattr__(self, "_c", (block, k, ks, v, vs))
+
+    def __reduce__(self):                              # (a copy, or a cache that comes out of a file, has other buffers and needs a block of its own)
+        return type(self), (self.k, self.k_scale, self.v, self.v_scale, self.elem)
 
     @property
     def num_kv_heads(self) -> int:
@@ -211,7 +214,8 @@ class KVCache:
         return self.k.shape[3] * (2 if self.elem == "e2m1" else 1)
 
     def _block(self) -> _Cache:
-        return _Cache.from_buffer_copy(self._c)
+        self.__post_init__()
+        return _Cache.from_buffer_copy(self._c[0])
 
 
 def kv_cache(num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64, elem: str = "e4m3", device="cuda") -> KVCache:
@@ -250,7 +254,7 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     A block's scale is the smallest power of two at which no element exceeds the type's largest value; a block with a NaN or an infinity
     reads back as NaN.  Pages written by one call must not be shared between its sequences."""
     if tensor_layout in ("HND", "NHD"):
-        r = _lib.native().kv_append(cache._c, cache.k, k, v, page_table, start, counts, tensor_layout == "HND")
+        r = _lib.native().kv_append(cache._c, k, v, page_table, start, counts, tensor_layout == "HND")
         if r is not None:
             return _lib.check(r)
     _require_cuda(k, v, page_table, start, counts)
@@ -278,7 +282,7 @@ def kv_cache_read(cache: KVCache, page_table: torch.Tensor, lengths: torch.Tenso
     on and where the table names no page.  max_len: all that the table can hold unless given.  For a prefill over a cached prefix
     (attention_forward takes them as k and v)."""
     if max_len is not None and out_dtype in _OUT_DTYPE:
-        r = _lib.native().kv_read(cache._c, cache.k, page_table, lengths, max_len, _OUT_DTYPE[out_dtype])
+        r = _lib.native().kv_read(cache._c, page_table, lengths, max_len, _OUT_DTYPE[out_dtype])
         if r is not None:
             if r.__class__ is int:
                 _lib.check(r)
@@ -316,7 +320,7 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     if st.word.value:
         _raise_if_failed(dev)
     if tensor_layout in ("HND", "NHD"):
-        r = _lib.native().kv_attention(cache._c, cache.k, q, page_table, lengths, q_lens, mask, st.status_ptr,
+        r = _lib.native().kv_attention(cache._c, q, page_table, lengths, q_lens, mask, st.status_ptr,
                                        cache.head_dim ** -0.5 if sm_scale is None else sm_scale, return_lse, tensor_layout == "HND")
         if r is not None:
             if r.__class__ is int:
