@@ -88,22 +88,36 @@ def grid_positions(grid, length: int, device=None) -> torch.Tensor:
     return pos
 
 
+_OTHER_NORMS = (torch.nn.LayerNorm, torch.nn.GroupNorm, torch.nn.modules.batchnorm._NormBase)
+
+
+def _rms_norm(norm, width: int, dtype):
+    """Weight and epsilon of an RMS norm over `width` elements; (None, 0) for an identity."""
+    if isinstance(norm, torch.nn.Identity):
+        return None, 0.0
+    weight, eps = getattr(norm, "weight", None), getattr(norm, "eps", getattr(norm, "variance_epsilon", "none"))
+    if eps is None and isinstance(norm, torch.nn.RMSNorm):
+        eps = torch.finfo(dtype).eps
+    if isinstance(norm, _OTHER_NORMS) or getattr(norm, "bias", None) is not None or weight is None or weight.numel() != width or not isinstance(eps, (int, float)):
+        raise ValueError("fused_norm_rope needs norm_q and norm_k to be RMS norms over all heads, with a weight, an epsilon and no bias, or identities")
+    return weight, eps
+
+
 def _wan_norm_rope(attn, q, k, grid_sizes, freqs):
     """norm_q, norm_k (RMS over all heads of a token) and rope_apply (pairs of neighbours; the table's columns split among frame, height and
-    width) of a Wan self-attention block in one pass; q, k [B,L,H,D]."""
+    width) of a Wan self-attention block in one pass, or one for each where the norms differ in more than their weights; q, k [B,L,H,D]."""
     from .serving import norm_rope
     L, d = q.shape[1], q.shape[3]
     half = d // 2
     side = half // 3
-    weights = [getattr(n, "weight", None) for n in (attn.norm_q, attn.norm_k)]
-    if any(w is None for w in weights) and not all(isinstance(n, torch.nn.Identity) for n in (attn.norm_q, attn.norm_k)):
-        raise ValueError("fused_norm_rope needs RMS norms with weights, or none")
-    normed = weights[0] is not None
+    (wq, eps_q), (wk, eps_k) = (_rms_norm(n, q.shape[2] * d, q.dtype) for n in (attn.norm_q, attn.norm_k))
     positions = torch.stack([grid_positions(g, L, q.device) for g in grid_sizes.tolist()])
     freqs = freqs.to(q.device)
-    return norm_rope(q, k, q_weight=weights[0], k_weight=weights[1], norm=normed, across_heads=normed, eps=float(getattr(attn.norm_q, "eps", 1e-6)),
-                     rope=(freqs.real.float().contiguous(), freqs.imag.float().contiguous()), positions=positions,
-                     sections=(half - 2 * side, side, side), interleaved=True, tensor_layout="NHD")
+    kw = dict(rope=(freqs.real.float().contiguous(), freqs.imag.float().contiguous()), positions=positions, sections=(half - 2 * side, side, side),
+              interleaved=True, tensor_layout="NHD")
+    if eps_q == eps_k and (wq is None) == (wk is None):
+        return norm_rope(q, k, q_weight=wq, k_weight=wk, norm=wq is not None, across_heads=wq is not None, eps=eps_q, **kw)
+    return tuple(norm_rope(x, q_weight=w, norm=w is not None, across_heads=w is not None, eps=e, **kw) for x, w, e in ((q, wq, eps_q), (k, wk, eps_k)))
 
 
 def _wan_self_attention_forward(rope_apply: Callable, fused: bool = False):
@@ -134,8 +148,9 @@ def set_mpsa_attn_wan(model, rope_apply: Optional[Callable] = None, block_scale_
     """Every block's self-attention of a Wan model (`model.blocks[i].self_attn` with q/k/v/o projections, norm_q/norm_k,
     num_heads, head_dim) computes its attention with this library from now on; returns the number of blocks patched.
     rope_apply: the model family's rotary function (default: wan.modules.model.rope_apply).
-    fused_norm_rope: norm_q, norm_k and the rotation of one block in one launch of this library's norm_rope, rounded once at the end
-    (rope_apply is then not called and not needed)."""
+    fused_norm_rope: norm_q, norm_k and the rotation of one block in one pass of this library's norm_rope, rounded once at the end
+    (rope_apply is then not called and not needed; the grid's positions and the table in fp32 are made anew in every block, a dozen small
+    launches).  norm_q and norm_k must be RMS norms over all heads, or identities; other norms raise ValueError."""
     if rope_apply is None and not fused_norm_rope:
         from wan.modules.model import rope_apply as _rope_apply      # the model's own package
         rope_apply = _rope_apply
