@@ -277,7 +277,8 @@ bool rows_aligned(const at::Tensor& t, int elements) {
          fits_int(t.size(2)) && fits_int(t.size(3));
 }
 
-bool asks_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// A gradient, or a tangent of forward mode (no_grad leaves those on)
+bool asks_gradient(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 
 // int32 [B], dense, on `device`
 bool indices(const at::Tensor& t, int64_t B, int device) {
@@ -363,7 +364,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((cos != nullptr) != (sin != nullptr) || (!cos && (pos || a[9] != Py_None))) Py_RETURN_NONE;
     if (cos) {
       for (const at::Tensor* t : {cos, sin})
-        if (t->dim() != 2 || t->scalar_type() != at::kFloat || t->sizes() != cos->sizes() || !t->is_contiguous() || t->get_device() != device || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16) Py_RETURN_NONE;
+        if (t->dim() != 2 || t->scalar_type() != at::kFloat || t->sizes() != cos->sizes() || !t->is_contiguous() || t->get_device() != device || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 || asks_gradient(*t)) Py_RETURN_NONE;
       if (!fits_int(cos->size(0)) || !fits_int(cos->size(1)) || 2 * cos->size(1) > c.D) Py_RETURN_NONE;
       c.cos = cos->data_ptr(); c.sin = sin->data_ptr();
       c.table_rows = cos->size(0); c.rot = (int)(2 * cos->size(1));

@@ -7,7 +7,7 @@ tokens, chunks or trees of drafted tokens over it.  The reference has none of th
     mpsa.kv_cache_append(cache, k, v, page_table, lengths)              # tokens lengths[b] .. lengths[b] + T - 1
     o = mpsa.kv_cache_attention(q, cache, page_table, lengths + T)      # the last T tokens of each sequence
 
-No gradients: these are inference operations, and operands that ask for one are refused.
+No gradients: these are inference operations, and operands that ask for one, or have tangents of forward mode, are refused.
 """
 from __future__ import annotations
 
@@ -16,6 +16,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _IN_DTYPE, _OUT_DTYPE, _bhld, _on_device, _ptr, _raise_if_failed, _require_cuda, _state
@@ -65,6 +66,8 @@ def _aligned(x: torch.Tensor, tensor_layout: str, elements: int):
 def _no_gradient(*ts):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise ValueError("no gradient is computed here: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):       # (no_grad() leaves these on)
+        raise ValueError("no derivative is computed here: operands have tangents")
 
 
 def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Optional[torch.Tensor] = None,
@@ -90,7 +93,7 @@ def norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, q_weight: Op
             _lib.check(r)
         return r
     _require_cuda(q, k, q_weight, k_weight, positions)
-    _no_gradient(q, k, q_weight, k_weight)
+    _no_gradient(q, k, q_weight, k_weight, *(() if rope is None else rope))
     if q.dtype not in _IN_DTYPE:
         raise ValueError(f"unsupported input dtype {q.dtype}")
     a = _NormRopeArgs()
