@@ -282,8 +282,11 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
 def kv_cache_read(cache: KVCache, page_table: torch.Tensor, lengths: torch.Tensor, *, max_len: Optional[int] = None,
                   out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values of whole sequences in out_dtype (bf16, fp16, fp32): two tensors [B, Hkv, max_len, D], zero from lengths[b]
-    on and where the table names no page.  max_len: all that the table can hold unless given.  For a prefill over a cached prefix
-    (attention_forward takes them as k and v)."""
+    on and where the table names no page.  max_len: all that the table can hold unless given.
+
+    For a prefill over a cached prefix, attention_forward takes them as k and v.  It knows no lengths (a zero row is a key like any other, and
+    causality is counted from the end): in one call with max_len the length that all sequences have, and for a ragged batch a sequence at a time,
+    k[b:b+1, :, :n], v[b:b+1, :, :n] with n = lengths[b].  kv_cache_attention takes ragged batches as they are."""
     if max_len is not None and out_dtype in _OUT_DTYPE:
         r = _lib.native().kv_read(cache._c, page_table, lengths, max_len, _OUT_DTYPE[out_dtype])
         if r is not None:
