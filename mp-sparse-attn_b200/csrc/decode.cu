@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(32 * kWarps, per_sm(NR, ELEM, D)) kv_attention
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kSet;
             if (top > m[n][x]) {
               const float f = exp2_fast(m[n][x] - top);
-              l[n][x] *= f;
+              l[n][x] = lowered(l[n][x], m[n][x] - top);
 #pragma unroll
               for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(32 * kWarps, per_sm(NR, ELEM, D)) kv_attention
       for (int w = 0; w < kWarps; ++w) {
         const float f = exp2_fast(row_stat[w][r].x - ref);
         const float4 y = *reinterpret_cast<const float4*>(merge + (w * Y::rows + r) * Y::pitch + d);
-        sum += f * row_stat[w][r].y;
+        sum += lowered(row_stat[w][r].y, row_stat[w][r].x - ref);
         v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
       }
       if constexpr (CLUSTER) {                        // (the place of warp 0's part: nobody else reads it)
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(32 * kWarps, per_sm(NR, ELEM, D)) kv_attention
           const float2 st = load_cluster2(at_rank(stats + r * 8, c));
           const float4 y = load_cluster4(at_rank(parts + (r * Y::pitch + d) * 4, c));
           const float f = exp2_fast(st.x - ref);
-          sum += f * st.y;
+          sum += lowered(st.y, st.x - ref);
           v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
         }
         write_out<T>(a, b, h, G, row0 + r, ql, d, v, top, sum);
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv_combine_kernel(const __grid_co
   for (int i0 = 0; i0 < parts; i0 += 32) {
     const float2 st = i0 == 0 ? first : i0 + lane < parts ? a.stat[slot(i0 + lane)] : nothing;
     const float f = exp2_fast(st.x - ref);
-    sum += f * st.y;
+    sum += lowered(st.y, st.x - ref);
     const int n = min(parts - i0, 32);
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {

@@ -63,6 +63,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// A denominator relative to a reference 2^-d as large, d at most 0 (-infinity with l = 0).  In two steps where 2^d is no number: keys without values
+// set a reference that may be 2^-200 of another's, and their denominators are as much larger.
+__device__ __forceinline__ float lowered(float l, float d) {
+  const float a = fmaxf(d, -100.0f);
+  return l * exp2_fast(a) * exp2_fast(d - a);
+}
+
 // Many query rows (csrc/decode_wide.cu): launches the kernel that leaves whole units in a.out and parts in a.part, a.stat.
 constexpr int kWideRows = 128, kWideStep = 128, kWideCtas = 2;       // CTAs of an SM
 int launch_wide(const Call& a, int ctas, cudaStream_t st);

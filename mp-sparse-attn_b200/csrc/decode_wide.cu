@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
                   tmem_st16(mine + 128 + 16 * i, x);
                 }
               }
-              l *= w;
+              if (raise) l = lowered(l, U - up);
               U = up;
             }
             const float ref = U == -INFINITY ? 0.0f : U;

@@ -236,3 +236,23 @@ def test_keys_and_values_of_all_sizes(elem, T):
     q = rnd(g, 1, Hq, T, D)
     out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
     check_by_key(c, table, n, q, out.cpu(), lse.cpu())
+
+
+@pytest.mark.parametrize("place", [2, 250, 19000])
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("elem", ["e4m3", "e5m2", "e2m1"])
+def test_keys_without_values_beside_one_with_large_ones(elem, T, place):
+    """All values are zero but those of one key, which are 2^60: every key has its weight, where a warp, a CTA or a part of the keys has seen nothing but
+    zeros, too."""
+    import mpsa
+    g = torch.Generator().manual_seed(place)
+    D, Hq = 64, 2
+    for n in (300, 20000):
+        if place >= n - T:
+            continue
+        k, v = rnd(g, 1, 1, n, D), torch.zeros(1, 1, n, D, dtype=BF16)
+        v[0, 0, place] = 2.0 ** 60
+        c, table = cache_of_rows(g, k, v, elem)
+        q = rnd(g, 1, Hq, T, D, amp=0.5)
+        out, lse = mpsa.kv_cache_attention(q.cuda(), c, table.cuda(), i32(n), return_lse=True)
+        check_attention(c, table, [n], q, out.cpu(), lse.cpu())
