@@ -161,20 +161,21 @@ __device__ __forceinline__ void request(Rows<ELEM, D>& r, const void* codes, con
   }
 }
 
-// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by, negative ones by 2^-24 once
-// more; base: the scale code of key `lane` that stands for 2^kUp; nan: what a NaN scale becomes.
+// fp16 rows into shared memory.  factors (shared memory of the warp): what the blocks of each key are multiplied by; base: the scale code of key
+// `lane` that stands for 2^kUp; nan: what a NaN scale becomes.
 template <int ELEM, int D>
 __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, int row0, uint32_t factors, int base, uint32_t nan, int lane) {
   using R = Rows<ELEM, D>;
   constexpr int NB = D / 32;
   uint32_t f[4] = {};
+  // E5M2: codes reach 2^16, and a factor below 2^-24 would be nothing where the product is not yet.  Such blocks are multiplied twice.
+  bool again = false;
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const uint32_t e = r.scale >> (8 * i) & 255u;
     const int d = (int)e - base + kUp<ELEM>;
-    f[i] = e == 255u ? nan : power2(d);
-    if constexpr (ELEM == E5M2)                        // (codes reach 2^16: the factor would be nothing where the product is not yet)
-      if (e != 255u && d < -24) f[i] = power2(d + 24) | 0x80008000u;
+    f[i] = e == 255u ? nan : power2(ELEM == E5M2 && e >= 2u ? max(d, -24) : d);
+    if (ELEM == E5M2) again |= d < -24 && e >= 2u;
   }
   __syncwarp();
   store_shared16(factors + 16 * lane, f[0], f[1], f[2], f[3]);
@@ -200,13 +201,26 @@ __device__ __forceinline__ void convert(const Rows<ELEM, D>& r, uint32_t tile, i
         elem_two<ELEM>(w[2 * j], x[0], x[1]);
         elem_two<ELEM>(w[2 * j + 1], x[2], x[3]);
       }
+      store_shared16((first ^ (16 * j + (R::rpi == 4 ? i % 2 * 64 : 0))) + i * R::rpi * 128, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
+    }
+  }
+  if (ELEM == E5M2 && __any_sync(0xffffffffu, again)) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y) x[y] = times(x[y], m);
-      if constexpr (ELEM == E5M2)
-        if (m & 0x8000u)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) x[y] = times(x[y], 0x80018001u);          // -2^-24
-      store_shared16((first ^ (16 * j + (R::rpi == 4 ? i % 2 * 64 : 0))) + i * R::rpi * 128, x[0], x[1], x[2], x[3]);
+    for (int i = 0; i < NB; ++i) {
+      const uint32_t e = r.scale >> (8 * i) & 255u;
+      f[i] = power2(e >= 2u && e < 255u ? min((int)e - base + kUp<ELEM> + 24, 0) : 0);
+    }
+    __syncwarp();
+    store_shared16(factors + 16 * lane, f[0], f[1], f[2], f[3]);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < R::cpr * out; ++i) {           // (each lane what it has written itself)
+      const int n = i / out;
+      const uint32_t at = (first ^ (16 * (i % out) + (R::rpi == 4 ? n % 2 * 64 : 0))) + n * R::rpi * 128;
+      uint32_t m, x[4];
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(m) : "r"(mul + n * R::rpi * 16) : "memory");
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+      store_shared16(at, times(x[0], m), times(x[1], m), times(x[2], m), times(x[3], m));
     }
   }
 }
@@ -566,27 +580,30 @@ __global__ void __launch_bounds__(kThreads, kWideCtas) kv_attention_wide_kernel(
       later = entry_of(as + 2);
       look_up();
       if (now) {
-        if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
         // One reference for the warp's keys of K where they are alike, one for each key of V, and for each of K otherwise: a key that a row
         // does not see, or gives no weight, may be larger than the rest by far.  (Codes 0 and 1 are blocks of nothing: no element reaches 2^-110.)
-        uint32_t top = 0, low = 255;
+        uint32_t own = 0, low = 255;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const uint32_t e = k.scale >> (8 * i) & 255u, d = v.scale >> (8 * i) & 255u;
-          top = max(top, e == 255u ? 0u : e);
+          const uint32_t e = k.scale >> (8 * i) & 255u;
+          own = max(own, e == 255u ? 0u : e);
           low = min(low, e < 2u ? 255u : e);
-          vtop = max(vtop, d == 255u ? 0u : d);
-          const uint32_t strange = __ballot_sync(0xffffffffu, d == 255u);
+        }
+        const uint32_t top = __reduce_max_sync(0xffffffffu, own);
+        const bool uneven = __any_sync(0xffffffffu, low + kSpread<ELEM> < top);
+        if (uneven) sh.k_part[par][32 * w + lane] = __uint_as_float((uint32_t)max(127 - (int)(top - own), 0) << 23);
+        if (n > 0 && !(ok = mbar_wait(&sh.s_full, (n - 1) & 1, a.status, KS_TIMEOUT_MMA))) break;      // K is free
+        convert<ELEM, D>(k, kt, 32 * w, factors, (int)(uneven ? own : top), 0x7fff7fffu, lane);
+        // (the scales of V were requested last: they have had K's conversion to come in)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const uint32_t e = v.scale >> (8 * i) & 255u;
+          vtop = max(vtop, e == 255u ? 0u : e);
+          const uint32_t strange = __ballot_sync(0xffffffffu, e == 255u);
           if (lane == 0) sh.strange[par][w][i] = strange;
         }
-        const uint32_t own = top;
-        top = __reduce_max_sync(0xffffffffu, top);
-        low = __reduce_min_sync(0xffffffffu, low);
-        const bool uneven = (int)top - (int)low > kSpread<ELEM>;
-        if (uneven) sh.k_part[par][32 * w + lane] = __uint_as_float((uint32_t)max(127 - (int)(top - own), 0) << 23);
         sh.v_size[par][32 * w + lane] = scale_value(vtop);
         sh.v_log[par][32 * w + lane] = fmaxf((float)((int)vtop - 127), kLeast);
-        convert<ELEM, D>(k, kt, 32 * w, factors, (int)(uneven ? own : top), 0x7fff7fffu, lane);
         const uint32_t has = __ballot_sync(0xffffffffu, here);
         if (lane == 0) {
           sh.there[par][w] = has;
