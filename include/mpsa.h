@@ -348,8 +348,12 @@ typedef struct mpsa_kv_read_args {
 } mpsa_kv_read_args;
 int mpsa_kv_read(const mpsa_kv_read_args* args, void* stream);
 
-/* Attention of the last tokens of each sequence over the cache that holds them: softmax(q k^T sm_scale) v in fp32 over the cached values,
- * P rounded to fp16.  Sequence b has lengths[b] keys, of which the last q_lens[b] (null: T) belong to its queries.  A query sees every key before those; of
+/* Attention of the last tokens of each sequence over the cache that holds them: softmax(q k^T sm_scale) v in fp32 over the cached values.
+ * Rounded to less: P times V's block scale (with more than 32 query rows of a KV head, the largest of its key), to fp16 with 11 bits down to
+ * 2^-21 of the row's largest such product and 2^-32 of it each below that; query elements below 2^-14 of their row's largest, to 2^-25 of it; and
+ * with more than 32 rows the blocks of a key of K or V that lie 2^22 (E5M2 2^8) or more below its largest, to 2^-31 of that.  Denominators are fp32 sums of P,
+ * whatever the values are.  Values from 2^-90 to 2^110 (outside, P has fewer bits); element codes are finite numbers, as mpsa_kv_append writes
+ * them.  Sequence b has lengths[b] keys, of which the last q_lens[b] (null: T) belong to its queries.  A query sees every key before those; of
  * those, query i sees key j iff j <= i, or with a mask iff mask[b,i,j] != 0.
  *   q, out    [B,Hq,T,D], 16-bit, element strides, innermost dense (q: strides multiples of 8, 16-byte aligned; out the same)
  *   mask      bytes [B or 1, T, T], batch stride mask_sb, dense rows

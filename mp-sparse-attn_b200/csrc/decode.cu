@@ -9,16 +9,19 @@
 //             that block.  Queries are brought to a largest magnitude of 1 .. 2 by a power of two of their row, so that their 8 or 11
 //             significant bits survive in fp16.
 //   output    O^T = V^T P^T, depth in the M dimension.  The block scales of V differ from key to key, so they go to P: for each block of the
-//             depth P times the scales is rounded to fp16 and multiplied by the codes.  This rounding of P is the only one below fp32.
+//             depth P times the scales is rounded to fp16 and multiplied by the codes.  This rounding of P, and that of query elements below
+//             2^-14 of their row's largest (2^-17 where they come in bf16), are the only ones below fp32.
 //   softmax   against a reference U of the row that keeps those products, not P, within fp16: U is set so that the largest (score plus log2
 //             of the key's largest scale) gives 2^7, and raised when one would give more than 2^15.  Products keep 11 bits down to 2^-21 of
 //             the row's largest, whatever the sizes of other keys' values are.  P and the row's sum of P are fp32; U is at least the largest
-//             score - 100, so that they stay finite (values below 2^-90 have fewer bits, then).
+//             score - 100, so that they stay finite (values below 2^-90 have fewer bits, then).  Weights below 2^-126 in units of U are dropped: beside
+//             values of 2^110 or more, where U is that much above the scores, they would matter.
 // Fragments of K and V come from ldmatrix on the codes as they are (.trans for V: two keys of neighbouring depth elements in a register).
 //
-// It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each.  8 KV heads of depth 128,
+// It is bound by the cache's bytes (HBM) as long as the conversions keep up: ALU-pipe instructions, two elements each; in E2M1, with twice the
+// elements a byte, by latency before any one pipe (issue and ALU 62 %, DRAM 50 %, 16 warps an SM).  8 KV heads of depth 128,
 // 4 query heads each: 32 sequences of up to 16384 tokens in E4M3 111 us (5.1 - 5.8 TB/s; 705 instructions a step and warp), 4 of 131072 in E2M1
-// 147 us (3.9 TB/s; ALU 62 %).  With queries in the M dimension the first took 140 us: half of each instruction's 16 rows were padding.
+// 147 us (3.9 TB/s).  With queries in the M dimension the first took 140 us: half of each instruction's 16 rows were padding.
 #include "api_internal.h"
 #include "decode.cuh"
 

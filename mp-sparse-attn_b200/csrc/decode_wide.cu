@@ -9,15 +9,16 @@
 //             Both lie as rows of 128 bytes, 128-byte swizzle: K is a K-major operand, V, untransposed, an MN-major one.
 //   Q K^T     128 x 128 x D, fp16 in, fp32 in TMEM.  Queries are scaled by a power of two of their row, as in decode.cu.
 //   softmax   a thread a row: P times V's factor, rounded to fp16, goes over S; the reference U keeps that within fp16 as decode.cu says
-//             (there it is each block's own scale).  One factor for 32 keys was no faster, and took bits from all others where a key without
-//             weight had large values.  The denominator adds up P itself: a key whose values are nothing,
-//             and whose product is, has its weight in it.  Steps in which every row sees every key (and K is alike) are tried against
-//             the references as they are, in one pass; where a product gets too large, and in the other steps, a pass over the scores finds the
-//             largest one first.
+//             (there it is each block's own scale).  One factor for 32 keys was 4 % faster, and took bits from all others where a key without
+//             weight had large values.  The denominator adds up P itself: a key whose values are nothing, and whose product is, has its weight
+//             in it.  Steps in which every row sees every key (and K is alike) are tried against the references as they are, in one pass;
+//             where a product gets too large, and in the other steps, a pass over the scores finds the largest one first.
 //   P V       128 x D x 128, P from TMEM, added up in TMEM.
 // One step is a chain (Q K^T, softmax, P V) but for the conversion of the next one; the two CTAs of an SM fill each other's gaps.
-// 8 sequences of up to 32768 tokens, 8 KV heads, trees of 32 tokens x 4 query heads: 156 - 202 us by box, 6300 cycles a step with two in flight on an SM:
-// softmax 2300, P V 850, Q K^T 1500 (operands and conversion share the shared-memory pipe), the rest hand-overs and what the conversion is late.
+// 8 sequences of up to 32768 tokens, 8 KV heads, trees of 32 tokens x 4 query heads: 177 - 186 us by box in E4M3, 179 in E5M2, 165 in E2M1.  7500 cycles a
+// step with two in flight on an SM: softmax 2650, P V 1500 and Q K^T 2300 with the wait for their operands.  The converting warps are never idle:
+// 950 and 800 cycles for the conversion of K and V, 2150 and 2000 until the loads of the next ones are issued, 900 for the look-ups.
+// (128 registers a thread, 56 - 96 bytes of which spill.)
 #include "api_internal.h"
 #include "decode.cuh"
 

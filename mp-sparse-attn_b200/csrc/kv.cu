@@ -1,6 +1,6 @@
 // The paged MX cache of keys and values: quantised as it is written (mpsa_kv_append) and read back (mpsa_kv_read).  See include/mpsa.h for
 // the layout.  Both are memory traffic: every element is read once and written once.  4 prefixes of 8192 tokens of 8 heads read back in 32 us
-// (5.9 TB/s); 2 x 4099 tokens appended in 12 us (4.2 TB/s: 16 loads and 60 ALU operations in 1.7 waves of CTAs).
+// (5.9 TB/s); 2 x 4099 tokens appended in 12 us (4.2 TB/s: 16 loads and 60 ALU operations, 2.3 waves of CTAs at 36 registers).
 #include "api_internal.h"
 #include "common.cuh"
 #include "serving.cuh"

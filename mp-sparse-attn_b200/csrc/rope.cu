@@ -1,6 +1,6 @@
 // RMS norm of queries and keys and their rotation by position in one pass (mpsa_norm_rope): every element is read once and written once.
 // Bound by HBM: 40 heads of 32768 tokens, each head's norm, 120 us (5.7 TB/s); 80 heads of 32760 tokens, norm across 40 heads, three axes,
-// 289 us (4.6 TB/s, issue 80 %).  A decoding step of 32 sequences takes the host's 7.8 us.
+// 276 - 289 us by box (4.6 - 4.9 TB/s, issue 71 %).  A decoding step of 32 sequences takes the host's 7.8 us.
 #include "api_internal.h"
 #include "common.cuh"
 #include "serving.cuh"

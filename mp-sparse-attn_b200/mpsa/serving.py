@@ -176,7 +176,7 @@ class KVCache:
 
     k, v uint8 [pages, Hkv, page_size, D] (elem "e4m3" or "e5m2") or [pages, Hkv, page_size, D/2] ("e2m1": two codes a byte, the lower depth
     in the low half); k_scale, v_scale uint8 [pages, Hkv, page_size, D/32]: an element stands for code * 2^(scale - 127), and a block with
-    the scale 255 for NaN.  A sequence's tokens lie in the pages that its row of a page table names; which pages it gets is the program's affair."""
+    the scale 255 for NaN (element codes are finite numbers).  A sequence's tokens lie in the pages that its row of a page table names; which pages it gets is the program's affair."""
     k: torch.Tensor
     k_scale: torch.Tensor
     v: torch.Tensor
@@ -320,7 +320,9 @@ def kv_cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor
     (the first ones; the rows behind them come back as zero); None: all, or lengths[b] where that is fewer.
     mask: bool [T,T] or [B,T,T], True where query token i sees query token j - a tree of drafted tokens; None: every token sees those before
     it and itself.  Cached tokens before the query tokens are seen by all.  A row that sees nothing is zero.
-    return_lse: also fp32 [B,Hq,T], log2 of the softmax denominators (-inf for a row that sees nothing), as attention_merge takes it."""
+    return_lse: also fp32 [B,Hq,T], log2 of the softmax denominators (-inf for a row that sees nothing), as attention_merge takes it.
+    Scores, weights and sums are fp32; a weight times its key's scale of v is rounded to fp16, relative to the largest one of the row.  What a key
+    does to a row goes by its own weight and size there, however large the keys beside it are."""
     dev = cache.k.device
     st = _state(dev.index)
     if st.word.value:
